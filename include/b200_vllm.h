@@ -135,6 +135,34 @@ void b200_dense_gemm_f16(const void* a, const void* w, void* c, int32_t m, int32
 void b200_dense_gemm_ex(const void* a, const void* w, const void* bias, void* c, int32_t m,
                         int32_t n, int32_t k, int32_t out_f32, int32_t mode, int64_t stream);
 
+/* ------------------------------------------------- linear layers in 8-bit integers (weights and activations)
+ * Rows to codes, a scale per row (the symmetric form of 8-bit checkpoints): out int8 [rows, width], scales fp32 [rows],
+ * value = code * scale, codes in [-127, 127].  q = round(127 t / max|t|), ties to even, exactly, with t = x, or x * weight behind
+ * an RMS norm (1 / rms is part of the scale only): codes are the same whatever the launch.  Any width.  A row of zeros has scale
+ * 0; a row with a NaN or an infinity has scale NaN and codes 0, so that what is computed from it is NaN.
+ * add_rmsnorm: residual += x first (rounded to 16 bits, as b200_add_rmsnorm_f16), then the norm of the residual.
+ * quant_rows also makes the weights' codes, a scale per output channel.                                            */
+void b200_rmsnorm_i8_f16(void* out, float* scales, const void* x, const void* weight, int32_t num_tokens,
+                         int32_t hidden, float eps, int64_t stream);
+void b200_rmsnorm_i8_bf16(void* out, float* scales, const void* x, const void* weight, int32_t num_tokens,
+                          int32_t hidden, float eps, int64_t stream);
+void b200_add_rmsnorm_i8_f16(void* out, float* scales, void* residual, const void* x, const void* weight,
+                             int32_t num_tokens, int32_t hidden, float eps, int64_t stream);
+void b200_add_rmsnorm_i8_bf16(void* out, float* scales, void* residual, const void* x, const void* weight,
+                              int32_t num_tokens, int32_t hidden, float eps, int64_t stream);
+void b200_quant_rows_i8_f16(void* out, float* scales, const void* x, int32_t rows, int32_t width, int64_t stream);
+void b200_quant_rows_i8_bf16(void* out, float* scales, const void* x, int32_t rows, int32_t width, int64_t stream);
+/* c[m, n] = (sum_k a[m, k] w[n, k]) * a_scales[m] * w_scales[n] (+ bias[n]): int8 a [m, k] and w [n, k], 16-byte aligned, k a
+ * multiple of 16 and at most 131056 (int32 sums stay exact for any codes), any m and n; fp32 epilogue, one rounding to the type
+ * of the suffix, which is bias's type too (bias may be NULL).  epilogue B200_EPI_SILU_MUL: w = gate rows, then as many up rows,
+ * c [m, n / 2] = silu(gate) * up of the fp32 values.  No workspace; results do not depend on the launch's shape.        */
+void b200_gemm_i8_f16(const void* a, const float* a_scales, const void* w, const float* w_scales, const void* bias,
+                      void* c, int32_t m, int32_t n, int32_t k, int32_t epilogue, int64_t stream);
+void b200_gemm_i8_bf16(const void* a, const float* a_scales, const void* w, const float* w_scales, const void* bias,
+                       void* c, int32_t m, int32_t n, int32_t k, int32_t epilogue, int64_t stream);
+void b200_gemm_i8_f32(const void* a, const float* a_scales, const void* w, const float* w_scales, const void* bias,
+                      void* c, int32_t m, int32_t n, int32_t k, int32_t epilogue, int64_t stream);
+
 /* ------------------------------------------------- RoPE + KV-cache write
  * Replaces FusedRope::apply_inplace (rotary_emb.rs:88-104) followed by the cache
  * write inside PagedAttention::forward (attention.rs:808-820) in ONE launch.

@@ -1,0 +1,336 @@
+"""8-bit integer linear layers against 64 bits.
+
+Codes are compared for equality: 127 t and A have at most 31 and 24 bits, so the 64-bit quotient is correctly rounded and exact
+where it is a tie.  Sums of products are exact in both; what is left is the fp32 epilogue, a rounding of 2^-24 per operation, and
+one rounding to the output's type, half a step of it."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+U = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def ops(lib):
+    from vllm_rs_b200 import ops as _ops
+    return _ops
+
+
+def _codes_of(t):
+    """(codes, maxima) of fp32 rows on the host, by the definition."""
+    bad = ~torch.isfinite(t).all(-1)
+    t64 = torch.where(bad[:, None], torch.zeros((), dtype=torch.float64), t.double())
+    top = t64.abs().amax(-1)
+    q = torch.round(t64 * 127.0 / torch.where(top > 0, top, torch.ones((), dtype=torch.float64))[:, None])
+    return q.to(torch.int8), torch.where(bad, torch.nan, top)
+
+
+def _check_rows(got, t, inv=None):
+    q, s = got[0].cpu(), got[1].cpu()
+    want, top = _codes_of(t)
+    assert torch.equal(q, want), f"{int((q != want).sum())} codes differ, first {(q != want).nonzero()[0].tolist()}"
+    scale = top / 127.0 if inv is None else top * inv / 127.0
+    nan = torch.isnan(scale)
+    assert torch.equal(torch.isnan(s), nan)
+    # plain: one division.  Norm: per thread at most 72 sums one after another, then 5 + 32 (half of it through the root), the
+    # root's two steps, three more operations: below 64 * 2^-24; the smallest fp32 step for scales below the normal range.
+    tol = (U if inv is None else 64 * U) * scale.abs() + 2.0 ** -149
+    assert bool(((s.double() - scale).abs() <= tol)[~nan].all())
+
+
+def _rows(seed, rows, width, dtype):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, width, generator=g) * (0.2 + 3 * torch.rand(rows, 1, generator=g))
+    x[torch.rand(rows, width, generator=g) < 0.01] *= 20
+    return x.to(dtype)
+
+
+def _inv(r, eps):
+    return (r.double().square().mean(-1) + eps).rsqrt()
+
+
+# widths on both sides of a piece of eight, of a warp, of 256 / 1024 / 4096 pieces per row and past what registers hold
+WIDTHS = [1, 2, 7, 8, 9, 31, 64, 100, 255, 256, 1000, 1024, 2047, 2048, 2056, 4096, 5632, 8192, 8200, 14336, 32768, 33001, 65600]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("width", WIDTHS)
+def test_rows(ops, width, dtype):
+    rows = 5 if width > 4096 else 37
+    x, r, w = _rows(width, rows, width, dtype), _rows(width + 1, rows, width, dtype), _rows(width + 2, 1, width, dtype)[0]
+    _check_rows(ops.quant_rows_i8(x.cuda()), x.float())
+    _check_rows(ops.rmsnorm_i8(x.cuda(), w.cuda(), 1e-5), x.float() * w.float(), _inv(x, 1e-5))
+    rd = r.cuda()
+    got = ops.add_rmsnorm_i8(rd, x.cuda(), w.cuda(), 1e-6)
+    total = (r.double() + x.double()).to(dtype)            # one rounding of the exact sum
+    assert torch.equal(rd.cpu(), total)
+    _check_rows(got, total.float() * w.float(), _inv(total, 1e-6))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("rows", [1, 2, 147, 148, 149, 1003, 5000])
+def test_many_rows(ops, rows, dtype):
+    for width in (128, 520, 2048):
+        x, w = _rows(rows, rows, width, dtype), _rows(width, 1, width, dtype)[0]
+        _check_rows(ops.quant_rows_i8(x.cuda()), x.float())
+        _check_rows(ops.rmsnorm_i8(x.cuda(), w.cuda(), 1e-5), x.float() * w.float(), _inv(x, 1e-5))
+
+
+def test_ties_and_their_neighbours(ops):
+    halves = torch.cat([torch.tensor([127.0, -127.0]), torch.arange(-126.5, 127.0)])                    # A = 127: every other border
+    odd = torch.cat([torch.tensor([254.0]), torch.arange(-253.0, 254.0, 2.0)])[:255]                    # A = 254
+    rows = [halves, odd, halves * 2.0 ** -20, halves * 2.0 ** -7]
+    x = torch.zeros(len(rows), 256)
+    for i, r in enumerate(rows):
+        x[i, :len(r)] = r
+    x = x.half()
+    _check_rows(ops.quant_rows_i8(x.cuda()), x.float())
+    want, _ = _codes_of(x.float())
+    assert want[0, 2:8].tolist() == [-126, -126, -124, -124, -122, -122]      # ties to even
+    # borders of other maxima, rounded to 16 bits, and the values next to them
+    for dtype in (F16, BF16):
+        g = torch.Generator().manual_seed(3)
+        top = (torch.rand(400, 1, generator=g) * 100 + 1).to(dtype).float()
+        near = ((torch.arange(127) + 0.5) * top / 127).to(dtype)
+        bits = near.view(torch.int16)
+        x = torch.cat([top.to(dtype)] + [(bits + d).view(dtype) for d in (-1, 0, 1)], 1)
+        x[:, 0] = torch.maximum(x[:, 0], x[:, 1:].amax(1))
+        _check_rows(ops.quant_rows_i8(x.cuda()), x.float())
+        w = _rows(5, 1, x.shape[1], dtype)[0]
+        _check_rows(ops.rmsnorm_i8(x.cuda(), w.cuda(), 1e-5), x.float() * w.float(), _inv(x, 1e-5))
+
+
+@pytest.mark.parametrize("width", [1, 37, 512, 40000])
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+def test_rows_of_zeros_and_not_finite(ops, dtype, width):
+    x = _rows(width, 9, width, dtype)
+    tiny = torch.finfo(dtype).tiny
+    x[0] = 0
+    x[1] = -0.0
+    x[2, width // 2] = torch.nan
+    x[3, width - 1] = torch.inf
+    x[4, 0] = -torch.inf
+    x[5] = torch.finfo(dtype).max
+    x[6] = tiny * torch.finfo(dtype).eps               # the smallest subnormal
+    x[7] = tiny
+    x[8] = 0
+    x[8, width - 1] = -tiny * torch.finfo(dtype).eps
+    _check_rows(ops.quant_rows_i8(x.cuda()), x.float())
+    q, s = ops.quant_rows_i8(x.cuda())
+    assert not q[:5].any() and s[:2].tolist() == [0.0, 0.0]
+    w = torch.ones(width, dtype=dtype)
+    y = x[torch.tensor([0, 1, 2, 3, 4, 7, 8])]
+    _check_rows(ops.rmsnorm_i8(y.cuda(), w.cuda(), 1e-5), y.float(), _inv(torch.nan_to_num(y.float(), 0, 0, 0), 1e-5))
+    y, w = _rows(1, 3, width, dtype), w.clone()        # a weight that is not finite
+    w[0] = torch.nan
+    got = ops.rmsnorm_i8(y.cuda(), w.cuda(), 1e-5)
+    assert bool(torch.isnan(got[1]).all()) and not got[0].any()
+
+
+@pytest.mark.parametrize("width", [64, 100, 1000])
+def test_rows_stay_in_their_tensors(ops, width):
+    """Results that begin anywhere, and what lies around them."""
+    x = _rows(2, 6, width, BF16)
+    for off in (0, 1, 3, 8):
+        pad_q = torch.full((6 * width + 64,), 77, dtype=torch.int8, device="cuda")
+        pad_s = torch.full((16,), 7.0, device="cuda")
+        q, s = pad_q[off:off + 6 * width].view(6, width), pad_s[off:off + 6]
+        xs = torch.cat([torch.zeros(off, dtype=BF16), x.flatten()]).cuda()[off:].view(6, width)
+        got = ops.quant_rows_i8(xs, out=q, scales=s)
+        assert got[0] is q and got[1] is s
+        _check_rows(got, x.float())
+        assert bool((pad_q[:off] == 77).all() and (pad_q[off + 6 * width:] == 77).all())
+        assert bool((pad_s[:off] == 7).all() and (pad_s[off + 6:] == 7).all())
+    assert ops.quant_rows_i8(torch.empty(0, width, dtype=F16, device="cuda"))[0].shape == (0, width)
+
+
+# ---------------------------------------------------------------- products
+def _int8(seed, *shape):
+    return torch.randint(-128, 128, shape, generator=torch.Generator().manual_seed(seed), dtype=torch.int8)
+
+
+def _case(m, n, k, dtype, bias, seed=0):
+    g = torch.Generator().manual_seed(seed + m + n + k)
+    a, w = _int8(m + 2 * n + k, m, k), _int8(n + 3 * k, n, k)
+    sa = (0.5 + torch.rand(m, generator=g)) / 64
+    sw = (0.5 + torch.rand(n, generator=g)) / (64 * k ** 0.5)
+    return a, sa, w, sw, torch.randn(n, generator=g).to(dtype) if bias else None
+
+
+def _check_product(y, a, sa, w, sw, bias, dtype, silu=False):
+    acc = a.double() @ w.double().t()                    # exact: below 2^53
+    p = acc * sa.double()[:, None] * sw.double()
+    b = torch.zeros(w.shape[0], dtype=torch.float64) if bias is None else bias.double()
+    v = p + b
+    off = 4 * U * (p.abs() + b.abs())                    # conversion of the sum, two scales, the bias
+    if silu:
+        n = w.shape[0] // 2
+        g, u, dg, du = v[:, :n], v[:, n:], off[:, :n], off[:, n:]
+        sig = torch.sigmoid(g)
+        want = g * sig * u
+        # |silu'| <= 1.1; exponential (2 steps of 2^-23), sum, division, product
+        off = 1.1 * dg * u.abs() + (g * sig).abs() * du + 1.1 * dg * du + 7 * U * want.abs()
+    else:
+        want = v
+    half = torch.finfo(dtype).eps / 2
+    tol = off + (0 if dtype == F32 else half * (want.abs() + off)) + torch.finfo(dtype).tiny * half
+    err = (y.double().cpu() - want).abs()
+    assert y.dtype == dtype and y.shape == want.shape
+    assert bool((err <= tol).all()), f"{int((err > tol).sum())} of {err.numel()} off, first {(err > tol).nonzero()[0].tolist()}"
+
+
+# rows around every tile edge, odd columns, K from one piece of 16 over ragged blocks of 128 to many of them
+SHAPES = [(1, 1, 16), (1, 128, 128), (1, 6144, 4096), (1, 1000, 272), (2, 7, 48), (3, 130, 1040), (4, 4096, 512), (5, 255, 4112),
+          (7, 1000, 256), (8, 129, 14336), (9, 64, 112), (15, 4096, 1024), (16, 300, 2048), (17, 2048, 144), (31, 96, 96), (32, 4096, 4096),
+          (33, 520, 640), (48, 1111, 1136), (63, 128, 256), (64, 2056, 2048), (65, 333, 528), (100, 1536, 4096), (127, 127, 128),
+          (128, 512, 896), (129, 256, 64), (160, 4096, 1024), (192, 77, 4096), (255, 640, 640), (256, 256, 256), (257, 4096, 2048),
+          (300, 1000, 512), (511, 384, 1152), (512, 4104, 512), (777, 1000, 3584), (1003, 2560, 1024), (2048, 1032, 528),
+          (4099, 515, 272)]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32], ids=["f16", "bf16", "f32"])
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_products(ops, m, n, k, dtype):
+    a, sa, w, sw, bias = _case(m, n, k, dtype, True)
+    c = [t.cuda() for t in (a, sa, w, sw)]
+    _check_product(ops.gemm_i8(*c, dtype=dtype), a, sa, w, sw, None, dtype)
+    _check_product(ops.gemm_i8(*c, bias=bias.cuda(), dtype=dtype), a, sa, w, sw, bias, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32], ids=["f16", "bf16", "f32"])
+@pytest.mark.parametrize("m,n,k", [(1, 2, 16), (1, 8192, 1024), (2, 200, 272), (6, 1030, 128), (16, 4096, 2048), (32, 1024, 4096),
+                                   (33, 66, 144), (64, 2050, 512), (128, 768, 640), (200, 514, 384), (257, 2048, 1024), (1003, 1280, 528),
+                                   (2050, 4100, 256)])
+def test_gated_products(ops, m, n, k, dtype):
+    a, sa, w, sw, bias = _case(m, n, k, dtype, True)
+    sw = sw * 4
+    c = [t.cuda() for t in (a, sa, w, sw)]
+    _check_product(ops.gemm_i8(*c, dtype=dtype, epilogue=ops.EPI_SILU_MUL), a, sa, w, sw, None, dtype, True)
+    _check_product(ops.gemm_i8(*c, dtype=dtype, bias=bias.cuda(), epilogue=ops.EPI_SILU_MUL), a, sa, w, sw, bias, dtype, True)
+
+
+@pytest.mark.parametrize("m", [1, 32, 130, 300])
+def test_largest_sums(ops, m):
+    """Every product 128 * 128 at the longest K: 131056 * 16384 is still below 2^31, and so is its negative."""
+    k, n = 131056, 40
+    w = torch.full((n, k), -128, dtype=torch.int8)
+    one = torch.ones(m)
+    for v in (-128, 127):
+        a = torch.full((m, k), v, dtype=torch.int8)
+        y = ops.gemm_i8(a.cuda(), one.cuda(), w.cuda(), torch.ones(n).cuda(), dtype=F32)
+        assert bool((y.double().cpu() == float(torch.tensor(-128.0 * v * k, dtype=F32))).all())
+
+
+def test_scales_that_are_not_finite(ops):
+    a, sa, w, sw, _ = _case(40, 200, 256, F16, False)
+    sa[3], sa[5], sw[7] = torch.nan, 0.0, torch.nan
+    y = ops.gemm_i8(a.cuda(), sa.cuda(), w.cuda(), sw.cuda()).cpu()
+    want = torch.zeros(40, 200, dtype=torch.bool)
+    want[3], want[:, 7] = True, True
+    assert torch.equal(torch.isnan(y), want) and not y[5, :7].any()
+
+
+@pytest.mark.parametrize("m", [1, 5, 32, 100, 300])
+@pytest.mark.parametrize("n", [64, 130, 1000])
+def test_products_stay_in_their_tensors(ops, m, n):
+    """Results that begin off 16 bytes, and what lies around them."""
+    for dtype, silu in ((F16, False), (BF16, True), (F32, False), (F32, True)):
+        a, sa, w, sw, bias = _case(m, n, 144, dtype, True)
+        cols = n // 2 if silu else n
+        for off in (0, 1, 4):
+            pad = torch.full((m * cols + 300,), 77.0, dtype=dtype, device="cuda")
+            out = pad[off:off + m * cols].view(m, cols)
+            pb = torch.cat([torch.zeros(off, dtype=dtype), bias]).cuda()[off:]
+            ops.gemm_i8(a.cuda(), sa.cuda(), w.cuda(), sw.cuda(), bias=pb, dtype=dtype, out=out,
+                        epilogue=ops.EPI_SILU_MUL if silu else ops.EPI_NONE)
+            _check_product(out, a, sa, w, sw, bias, dtype, silu)
+            assert bool((pad[:off] == 77).all() and (pad[off + m * cols:] == 77).all())
+
+
+def test_scales_and_operands_that_begin_anywhere(ops):
+    """Scales off 16 bytes; rows of a larger batch."""
+    m, n, k = 37, 260, 272
+    a, sa, w, sw, _ = _case(m, n, k, BF16, False)
+    big_a, big_w = torch.cat([_int8(1, 3, k), a, _int8(2, 5, k)]).cuda(), torch.cat([_int8(3, 1, k), w, _int8(4, 2, k)]).cuda()
+    for off in (0, 1, 2, 3):
+        ps, pw = torch.cat([torch.zeros(off), sa]).cuda()[off:], torch.cat([torch.zeros(off), sw]).cuda()[off:]
+        _check_product(ops.gemm_i8(big_a[3:3 + m], ps, big_w[1:1 + n], pw, dtype=BF16), a, sa, w, sw, None, BF16)
+
+
+# ---------------------------------------------------------------- together
+@pytest.mark.parametrize("tokens", [1, 32, 300])
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+def test_feed_forward_of_a_layer(ops, tokens, dtype):
+    """Norm, gate | up, activation, down as a decoder layer runs them: each step against the formula on what the step before gave,
+    the whole near the same layer in 64 bits, and a captured graph's replays equal to the calls, on inputs of their own."""
+    width, ff = 512, 1408
+    g = torch.Generator().manual_seed(tokens)
+    gate_up, down = (torch.randn(2 * ff, width, generator=g) / width ** 0.5).to(dtype), (torch.randn(width, ff, generator=g) / ff ** 0.5).to(dtype)
+    norm = (1 + 0.2 * torch.randn(width, generator=g)).to(dtype)
+    wq, ws = ops.quant_rows_i8(gate_up.cuda())
+    dq, ds = ops.quant_rows_i8(down.cuda())
+    _check_rows((wq, ws), gate_up.float())
+    nd = norm.cuda()
+
+    def layer(residual, x):
+        q, s = ops.add_rmsnorm_i8(residual, x, nd, 1e-5)
+        h = ops.gemm_i8(q, s, wq, ws, dtype=dtype, epilogue=ops.EPI_SILU_MUL)
+        hq, hs = ops.quant_rows_i8(h)
+        return q, s, h, hq, hs, ops.gemm_i8(hq, hs, dq, ds, dtype=dtype)
+
+    r0, x0 = _rows(tokens, tokens, width, dtype), _rows(tokens + 1, tokens, width, dtype)
+    residual, x = r0.cuda(), x0.cuda()
+    q, s, h, hq, hs, y = layer(residual, x)
+    total = (r0.double() + x0.double()).to(dtype)
+    assert torch.equal(residual.cpu(), total)
+    _check_rows((q, s), total.float() * norm.float(), _inv(total, 1e-5))
+    _check_product(h, q.cpu(), s.cpu(), wq.cpu(), ws.cpu(), None, dtype, True)
+    _check_rows((hq, hs), h.cpu().float())
+    _check_product(y, hq.cpu(), hs.cpu(), dq.cpu(), ds.cpu(), None, dtype)
+    # against the layer that is not quantised: a code is off by half a step at most, 1 / sqrt(12) of a step in the mean, which gives
+    # an operand's relative error from its own scales.  Errors of rows and weights add in a product as squares; gate and up are
+    # each off so, the activation's slope |silu'| <= 1.1 against silu / g in the mean near 0.6: 4 (ex^2 + ew^2) covers both.
+    # 1.5: errors of the few largest rows do not average as evenly.
+    part = lambda s, v: float((s.double().square().mean() / 12 / v.double().square().mean()).sqrt())        # noqa: E731
+    deq = lambda q, s: q.float() * s[:, None]                                                               # noqa: E731
+    ex, ew, eh, ed = part(s, deq(q, s)), part(ws, deq(wq, ws)), part(hs, deq(hq, hs)), part(ds, deq(dq, ds))
+    bound = 1.5 * (4 * (ex ** 2 + ew ** 2) + eh ** 2 + ed ** 2) ** 0.5
+    ref = total.double() * _inv(total, 1e-5)[:, None] * norm.double()
+    gu = ref @ gate_up.double().t()
+    ref = (torch.nn.functional.silu(gu[:, :ff]) * gu[:, ff:]) @ down.double().t()
+    assert float((y.double().cpu() - ref).norm() / ref.norm()) < bound < 0.5
+    # captured
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        residual.copy_(r0)
+        layer(residual, x)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = layer(residual, x)
+    torch.cuda.current_stream().wait_stream(side)
+    for seed in (5, 6):
+        r1, x1 = _rows(seed, tokens, width, dtype).cuda(), _rows(seed + 7, tokens, width, dtype).cuda()
+        residual.copy_(r1)
+        x.copy_(x1)
+        graph.replay()
+        again = [t.clone() for t in got] + [residual.clone()]
+        eager = layer(r1, x1)
+        assert all(torch.equal(p, e) for p, e in zip(again, (*eager, r1)))
+
+
+def test_two_streams_at_once(ops):
+    """Calls on two streams share nothing: results are those of one after the other."""
+    cases = [_case(m, 2048, 1024, BF16, False, seed) for m, seed in ((32, 1), (300, 2))]
+    cases = [[t.cuda() for t in c[:4]] for c in cases]
+    want = [ops.gemm_i8(*c, dtype=BF16) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, (st, c) in enumerate(zip(streams, cases)):
+            with torch.cuda.stream(st):
+                got[i].append(ops.gemm_i8(*c, dtype=BF16))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, w) for ys, w in zip(got, want) for y in ys)

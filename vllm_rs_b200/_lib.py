@@ -158,6 +158,15 @@ _SIGS = {
     "b200_wna16_dequant_f16": (None, [c_vp] * 4 + [c_i32] * 5 + [c_i64]),
     "b200_dense_gemm_f16": (None, [c_vp] * 3 + [c_i32] * 4 + [c_i64]),
     "b200_dense_gemm_ex": (None, [c_vp] * 4 + [c_i32] * 5 + [c_i64]),
+    "b200_rmsnorm_i8_f16": (None, [c_vp] * 4 + [c_i32, c_i32, c_f32, c_i64]),
+    "b200_rmsnorm_i8_bf16": (None, [c_vp] * 4 + [c_i32, c_i32, c_f32, c_i64]),
+    "b200_add_rmsnorm_i8_f16": (None, [c_vp] * 5 + [c_i32, c_i32, c_f32, c_i64]),
+    "b200_add_rmsnorm_i8_bf16": (None, [c_vp] * 5 + [c_i32, c_i32, c_f32, c_i64]),
+    "b200_quant_rows_i8_f16": (None, [c_vp] * 3 + [c_i32, c_i32, c_i64]),
+    "b200_quant_rows_i8_bf16": (None, [c_vp] * 3 + [c_i32, c_i32, c_i64]),
+    "b200_gemm_i8_f16": (None, [c_vp] * 6 + [c_i32] * 4 + [c_i64]),
+    "b200_gemm_i8_bf16": (None, [c_vp] * 6 + [c_i32] * 4 + [c_i64]),
+    "b200_gemm_i8_f32": (None, [c_vp] * 6 + [c_i32] * 4 + [c_i64]),
     "b200_rope_kv_write_f16": (None, [c_vp] * 9 + [c_i32] * 8 + [c_i64]),
     "b200_rope_kv_write_bf16": (None, [c_vp] * 9 + [c_i32] * 8 + [c_i64]),
     "b200_rope_kv_write_fp8kv_f16": (None, [c_vp] * 9 + [c_i32] * 8 + [c_i64]),
