@@ -138,8 +138,8 @@ void b200_dense_gemm_ex(const void* a, const void* w, const void* bias, void* c,
 /* ------------------------------------------------- linear layers in 8-bit integers (weights and activations)
  * Rows to codes, a scale per row (the symmetric form of 8-bit checkpoints): out int8 [rows, width], scales fp32 [rows],
  * value = code * scale, codes in [-127, 127].  q = round(127 t / max|t|), ties to even, exactly, with t = x, or x * weight behind
- * an RMS norm (1 / rms is part of the scale only): codes are the same whatever the launch.  Any width.  A row of zeros has scale
- * 0; a row with a NaN or an infinity has scale NaN and codes 0, so that what is computed from it is NaN.
+ * an RMS norm (1 / rms is part of the scale only): codes are the same whatever the launch.  Any width up to 2^30.  A row of zeros
+ * has scale 0; a row with a NaN or an infinity has scale NaN and codes 0, so that what is computed from it is NaN.
  * add_rmsnorm: residual += x first (rounded to 16 bits, as b200_add_rmsnorm_f16), then the norm of the residual.
  * quant_rows also makes the weights' codes, a scale per output channel.                                            */
 void b200_rmsnorm_i8_f16(void* out, float* scales, const void* x, const void* weight, int32_t num_tokens,

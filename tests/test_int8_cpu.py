@@ -31,6 +31,7 @@ def test_rows_refuse(lib, suffix):
         _refused(lib, lambda: f("add_rmsnorm")(*p, 2, 64, eps, 0), b"add_rmsnorm_i8")
     _refused(lib, lambda: f("rmsnorm")(A, A, A, A, 2, 0, eps, 0), b"rmsnorm_i8")
     _refused(lib, lambda: f("quant_rows")(A, A, A, 2, 0, 0), b"quant_rows_i8")
+    _refused(lib, lambda: f("quant_rows")(A, A, A, 2, 2 ** 30 + 1, 0), b"quant_rows_i8")
     _refused(lib, lambda: f("quant_rows")(A, None, A, 2, 8, 0), b"quant_rows_i8")
     f("quant_rows")(None, None, None, 0, 8, 0)                           # no rows: nothing to do, nothing to refuse
     assert lib.b200_last_error() == 0
@@ -57,19 +58,14 @@ def test_gemm_refuses(lib, suffix):
 def ops(lib, monkeypatch):
     """The wrappers with tensors of the host: their checks run, a call that gets past them fails the test."""
     from vllm_rs_b200 import ops as o
-    real = o._cuda
-
-    def cuda(*ts):
-        for t in ts:
-            if t is not None and not t.is_contiguous():
-                raise ValueError("b200 ops need contiguous CUDA tensors")
+    def contiguous(*ts):
+        if not all(t is None or t.is_contiguous() for t in ts):
+            raise ValueError("not contiguous")
 
     def launched(*_):
         raise AssertionError("a call that should have been refused reached the library")
 
-    assert real is not cuda
-    monkeypatch.setattr(o, "_cuda", cuda)
-    monkeypatch.setattr(o, "_here", lambda *ts: None)
+    monkeypatch.setattr(o, "_on_device", contiguous)
     monkeypatch.setattr(o, "_stream", launched)
     return o
 
@@ -85,6 +81,14 @@ def test_wrappers_refuse_rows(ops):
             call()
     with pytest.raises(TypeError):
         ops.quant_rows_i8(x.float())
+
+
+def test_wrappers_refuse_tensors_of_the_host(lib, monkeypatch):
+    from vllm_rs_b200 import ops
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    x = torch.zeros(3, 64, dtype=torch.float16)
+    with pytest.raises(ValueError, match="current device"):
+        ops.quant_rows_i8(x)
 
 
 def test_wrappers_refuse_products(ops):

@@ -4,16 +4,26 @@
 //   t = x (plain) or x * w (norm);   A = max|t|;   scale = A / 127 (norm: A / (127 rms));   q = round(127 t / A)
 //
 // The norm's 1 / rms multiplies numerator and maximum alike, so it appears in the scale alone and one pass over the row gives
-// the sum of squares and the maximum together.  t is exact in fp32 (two 16-bit factors).  The quotient is rounded to the nearest
-// integer, ties to even, EXACTLY: fp32 decides unless it lies within 3e-5 of a border (its error is below 127 * 2^-23), then
-// 254 |t| is compared with (2 floor + 1) A in fp64, where both are exact.  So codes do not depend on how threads share a row.
+// the sum of squares and the maximum together.  t is exact in fp32 (two 16-bit factors).
+//
+// The quotient is rounded to the nearest integer, ties to even, EXACTLY, so codes do not depend on how threads share a row.
+// Where t has at most 16 bits, 127 t is exact and v = p / A comes from one Newton step on p (1 / A): correctly rounded but for
+// 2^-47.  A tie is a number of fp32 and comes out as itself; any other quotient is at least 1 / (254 * 2^16) > 2^-24 of its size
+// away from a tie, and stays on its side.  (fp16 data make ties common, bf16 data very common: one in some hundred where A is a
+// power of two, so they must not cost a branch.)  fp16 times fp16 has 22 bits: fp32 decides unless the quotient lies within 3e-5
+// of a border (its error is below 127 * 2^-23), then 254 |t| is compared with (2 floor + 1) A without rounding.
+//
 // A row of zeros has scale 0 and codes 0.  A row with a NaN or an infinity has scale NaN and codes 0: all that is computed from
-// it is NaN.  Maxima are taken over the bits, where every NaN is larger than infinity.
+// it is NaN.
 #include "../../include/b200_vllm.h"
 #include "common.cuh"
+#include "f32x2.cuh"
 
 namespace b200 {
 namespace rows8 {
+
+constexpr int kWarpRows = 8;        // rows of a block where each warp has one
+constexpr int kMaxWidth = 1 << 30;  // columns are counted in 32 bits
 
 struct Args {
   int8_t* out;
@@ -25,89 +35,190 @@ struct Args {
   float eps;
 };
 
-// How a row's codes follow from its maximum.
-struct Coder {
-  float mul, up, top;
-  __device__ __forceinline__ explicit Coder(float top_) : top(top_) {
-    up = top < 1e-30f ? 18446744073709551616.f : 1.f;        // 2^64: 127 / A would overflow (exact, as is t * up)
-    mul = top > 0.f ? 127.f / (top * up) : 0.f;
-  }
-  // the code in the low byte
-  __device__ __forceinline__ uint32_t operator()(float t) const {
-    constexpr float kMagic = 12582912.f;                       // 1.5 * 2^23: a sum with it is rounded to an integer
-    const float u = t * up;
-    float m = fmaf(u, mul, kMagic);
-    const float k = m - kMagic;
-    const float d = fabsf(fmaf(u, mul, -k));
-    if (d > 0.49997f) {
-      const float f = floorf(fabsf(u * mul));
-      const double lhs = 254.0 * fabs(static_cast<double>(t)), rhs = (2.0 * static_cast<double>(f) + 1.0) * static_cast<double>(top);
-      const bool odd = static_cast<int>(f) & 1;
-      const float r = lhs > rhs || (lhs == rhs && odd) ? f + 1.f : f;
-      m = copysignf(r, t) + kMagic;
-    }
-    return __float_as_uint(m);
-  }
-};
-
 __device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
-// Eight elements of a row from index i on.  VEC: 16-byte accesses (width a multiple of 8, all aligned).
-template <bool VEC>
-__device__ __forceinline__ uint4 load8(const uint16_t* p, int i, int width) {
-  if constexpr (VEC) {
-    return *reinterpret_cast<const uint4*>(p + i);
-  } else {
-    uint32_t h[4];
+// How a row's codes follow from its maximum A.  SHORT: t has at most 16 significant bits (all but fp16 behind a norm, which has 22).
+// Two elements per instruction.
+template <bool SHORT>
+struct Coder {
+  static constexpr float kMagic = 12582912.f;      // 1.5 * 2^23: a sum with it is rounded to an integer, its low byte the code
+  f2 inv, c127, minus_a;
+  float a, mul;
+  __device__ __forceinline__ explicit Coder(float top) {
+    // neither 127 t nor 1 / A may leave the normal range (fp16 never does)
+    const float up = top < 1e-30f ? 18446744073709551616.f : top > 1e30f ? 5.421010862427522e-20f : 1.f;       // 2^64, 2^-64
+    a = top * up;
+    const float r = top > 0.f ? 1.f / a : 0.f;
+    mul = 127.f * r;
+    inv = pack2(r, r);
+    c127 = pack2(127.f * up, 127.f * up);
+    minus_a = pack2(-a, -a);
+  }
+  // 254 |t| against (2 floor + 1) A: both split into a rounded and a remaining part, whose difference is exact next to a border
+  __device__ __forceinline__ float at_border(float t) const {
+    const float u = fabsf(t), f = floorf(u * mul), p = 254.f * u, pe = fmaf(254.f, u, -p);
+    const float e = fmaf(-(2.f * f + 1.f), a, p) + pe;
+    const bool odd = static_cast<int>(f) & 1;
+    return copysignf(e > 0.f || (e == 0.f && odd) ? f + 1.f : f, t);
+  }
+  // eight codes
+  __device__ __forceinline__ uint2 operator()(const f2 (&t)[4]) const {
+    const f2 magic = pack2(kMagic, kMagic);
+    float m[8];
+    if constexpr (SHORT) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t lo = i + 2 * j < width ? p[i + 2 * j] : 0u, hi = i + 2 * j + 1 < width ? p[i + 2 * j + 1] : 0u;
-      h[j] = lo | hi << 16;
+      for (int j = 0; j < 4; ++j) {
+        const f2 p = mul2(t[j], c127), v = mul2(p, inv);
+        unpack2(add2(fma2(fma2(v, minus_a, p), inv, v), magic), m[2 * j], m[2 * j + 1]);
+      }
+    } else {
+      const f2 mul_2 = pack2(mul, mul), minus = pack2(-1.f, -1.f);
+      float off[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const f2 v = fma2(t[j], mul_2, magic);
+        unpack2(v, m[2 * j], m[2 * j + 1]);
+        unpack2(fma2(t[j], mul_2, fma2(v, minus, magic)), off[2 * j], off[2 * j + 1]);
+      }
+      const float worst = max3(max3(fabsf(off[0]), fabsf(off[1]), fabsf(off[2])), max3(fabsf(off[3]), fabsf(off[4]), fabsf(off[5])),
+                               fmaxf(fabsf(off[6]), fabsf(off[7])));
+      if (worst > 0.49997f) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float lo, hi;
+          unpack2(t[j >> 1], lo, hi);
+          if (fabsf(off[j]) > 0.49997f) m[j] = at_border(j & 1 ? hi : lo) + kMagic;
+        }
+      }
     }
-    return make_uint4(h[0], h[1], h[2], h[3]);
+    uint32_t b[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) b[j] = __float_as_uint(m[j]);
+    return make_uint2(low_bytes(b[0], b[1], b[2], b[3]), low_bytes(b[4], b[5], b[6], b[7]));
+  }
+};
+
+// Eight neighbours at any address (that of 16-bit elements: even): the widest accesses that its alignment allows.  All threads of a
+// row are eight elements apart and take the same branch.
+__device__ __forceinline__ uint4 load8_any(const uint16_t* p) {
+  const uint32_t mis = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p));
+  if ((mis & 15) == 0) return *reinterpret_cast<const uint4*>(p);
+  if ((mis & 7) == 0) {
+    const uint2 lo = *reinterpret_cast<const uint2*>(p), hi = *reinterpret_cast<const uint2*>(p + 4);
+    return make_uint4(lo.x, lo.y, hi.x, hi.y);
+  }
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(p + ((mis >> 1) & 1));
+  if ((mis & 3) == 0) return make_uint4(w[0], w[1], w[2], w[3]);
+  const uint32_t first = p[0], last = p[7], a = w[0], b = w[1], c = w[2];
+  return make_uint4(first | a << 16, __funnelshift_l(a, b, 16), __funnelshift_l(b, c, 16), c >> 16 | last << 16);
+}
+__device__ __forceinline__ void store8_any(uint16_t* p, const uint4& v) {
+  const uint32_t mis = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p));
+  if ((mis & 15) == 0) {
+    *reinterpret_cast<uint4*>(p) = v;
+  } else if ((mis & 3) == 0) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(p);
+    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+  } else {
+    uint32_t* w = reinterpret_cast<uint32_t*>(p + 1);
+    p[0] = static_cast<uint16_t>(v.x);
+    w[0] = __funnelshift_l(v.x, v.y, 16);
+    w[1] = __funnelshift_l(v.y, v.z, 16);
+    w[2] = __funnelshift_l(v.z, v.w, 16);
+    p[7] = static_cast<uint16_t>(v.w >> 16);
   }
 }
-template <bool VEC>
-__device__ __forceinline__ void store8(uint16_t* p, int i, int width, const uint4& v) {
-  if constexpr (VEC) {
-    *reinterpret_cast<uint4*>(p + i) = v;
+__device__ __forceinline__ void store8_any(int8_t* p, const uint2& q) {
+  const uint32_t mis = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 7;
+  uint8_t* b = reinterpret_cast<uint8_t*>(p);
+  if (mis == 0) {
+    *reinterpret_cast<uint2*>(b) = q;
+  } else if (mis == 4) {
+    reinterpret_cast<uint32_t*>(b)[0] = q.x;
+    reinterpret_cast<uint32_t*>(b)[1] = q.y;
+  } else if ((mis & 1) == 0) {
+    *reinterpret_cast<uint16_t*>(b) = static_cast<uint16_t>(q.x);
+    *reinterpret_cast<uint32_t*>(b + 2) = __funnelshift_l(q.x, q.y, 16);
+    *reinterpret_cast<uint16_t*>(b + 6) = static_cast<uint16_t>(q.y >> 16);
+  } else if ((mis & 3) == 3) {
+    b[0] = static_cast<uint8_t>(q.x);
+    *reinterpret_cast<uint32_t*>(b + 1) = __funnelshift_r(q.x, q.y, 8);
+    *reinterpret_cast<uint16_t*>(b + 5) = static_cast<uint16_t>(q.y >> 8);
+    b[7] = static_cast<uint8_t>(q.y >> 24);
   } else {
-    const uint32_t h[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (i + j < width) p[i + j] = static_cast<uint16_t>(h[j >> 1] >> (16 * (j & 1)));
-  }
-}
-template <bool VEC>
-__device__ __forceinline__ void store8(int8_t* p, int i, int width, uint32_t lo, uint32_t hi) {
-  if constexpr (VEC) {
-    *reinterpret_cast<uint2*>(p + i) = make_uint2(lo, hi);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (i + j < width) p[i + j] = static_cast<int8_t>((j < 4 ? lo : hi) >> (8 * (j & 3)));
+    b[0] = static_cast<uint8_t>(q.x);
+    *reinterpret_cast<uint16_t*>(b + 1) = static_cast<uint16_t>(q.x >> 8);
+    *reinterpret_cast<uint32_t*>(b + 3) = __funnelshift_r(q.x, q.y, 24);
+    b[7] = static_cast<uint8_t>(q.y >> 24);
   }
 }
 
-// The values t of eight elements; the sum of squares and the bits of the maximum so far take them in.
+// Thread `tid` of `n` that share a row: piece c of it, eight neighbours.  VEC: the width is a multiple of 8 and all begins on 16 bytes
+// (codes: on eight); else the row's last piece goes element by element.
+template <bool VEC>
+struct Piece {
+  int at, width;
+  __device__ __forceinline__ Piece(int tid, int c, int n, int width_) : at((c * n + tid) * 8), width(width_) {}
+  __device__ __forceinline__ uint4 load(const uint16_t* p) const {
+    if constexpr (VEC) {
+      return at < width ? *reinterpret_cast<const uint4*>(p + at) : make_uint4(0, 0, 0, 0);
+    } else {
+      if (at + 8 <= width) return load8_any(p + at);
+      uint32_t h[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) h[j] = at + j < width ? p[at + j] : 0u;
+      return make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+    }
+  }
+  __device__ __forceinline__ void store(uint16_t* p, const uint4& v) const {
+    if constexpr (VEC) {
+      if (at < width) *reinterpret_cast<uint4*>(p + at) = v;
+    } else if (at + 8 <= width) {
+      store8_any(p + at, v);
+    } else {
+      const uint32_t h[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (at + j < width) p[at + j] = static_cast<uint16_t>(h[j >> 1] >> (16 * (j & 1)));
+    }
+  }
+  __device__ __forceinline__ void store(int8_t* p, const uint2& q) const {
+    if constexpr (VEC) {
+      if (at < width) *reinterpret_cast<uint2*>(p + at) = q;
+    } else if (at + 8 <= width) {
+      store8_any(p + at, q);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (at + j < width) p[at + j] = static_cast<int8_t>((j < 4 ? q.x : q.y) >> (8 * (j & 3)));
+    }
+  }
+};
+
+// max(|a|, |b|, |c|), NaN where one is
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// The values t of eight elements; the sum of squares and the maximum so far take them in.
 template <bool BF, bool NORM>
-__device__ __forceinline__ void take8(const uint4& a, const uint4& w, float (&t)[8], float& ss, uint32_t& top) {
+__device__ __forceinline__ void take8(const uint4& a, const uint4& w, f2 (&t)[4], f2& ss, float& top) {
   const uint32_t ah[4] = {a.x, a.y, a.z, a.w}, wh[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    float2 f = unpack16x2<BF>(ah[j]);
+    const float2 f = unpack16x2<BF>(ah[j]);
+    t[j] = pack2(f.x, f.y);
     if constexpr (NORM) {
       const float2 g = unpack16x2<BF>(wh[j]);
-      ss = fmaf(f.x, f.x, ss);
-      ss = fmaf(f.y, f.y, ss);
-      f.x *= g.x;
-      f.y *= g.y;
+      ss = fma2(t[j], t[j], ss);
+      t[j] = mul2(t[j], pack2(g.x, g.y));
     }
-    t[2 * j] = f.x;
-    t[2 * j + 1] = f.y;
-    top = max(top, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
+    float lo, hi;
+    unpack2(t[j], lo, hi);
+    top = max3_abs(top, lo, hi);
   }
 }
 template <bool BF>
@@ -119,93 +230,121 @@ __device__ __forceinline__ uint4 add8(uint4 a, const uint4& r) {
   return a;
 }
 
-// A block per row, NC pieces of eight elements per thread (0: as many as it takes, read twice).
-template <bool BF, bool NORM, bool ADD, bool VEC, int NC>
-__global__ void rows_i8_kernel(const Args a) {
+// A block per row, or (WARP) a warp, NC pieces of eight elements per thread (0: as many as it takes, read twice).
+template <bool BF, bool NORM, bool ADD, bool VEC, bool WARP, int NC>
+__global__ void __launch_bounds__(WARP ? 32 * kWarpRows : NC ? 512 : 1024) rows_i8_kernel(const Args a) {
   pdl_trigger();
   pdl_wait();
-  __shared__ float red_ss[32];
-  __shared__ uint32_t red_top[32];
-  const size_t at = static_cast<size_t>(blockIdx.x) * a.width;
+  __shared__ float red_ss[WARP ? 1 : 32];
+  __shared__ uint32_t red_top[WARP ? 1 : 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row = WARP ? blockIdx.x * kWarpRows + warp : blockIdx.x, tid = WARP ? lane : threadIdx.x, n = WARP ? 32 : blockDim.x;
+  if (WARP && row >= a.rows) return;
+  const size_t at = static_cast<size_t>(row) * a.width;
   const uint16_t* x = a.x + at;
   uint16_t* res = ADD ? a.residual + at : nullptr;
   int8_t* out = a.out + at;
-  const int step = blockDim.x * 8, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float ss = 0.f;
-  uint32_t top = 0;
+  f2 squares = pack2(0.f, 0.f);
+  float most = 0.f;
 
-  auto fetch = [&](int i, float (&t)[8]) {
-    uint4 v = load8<VEC>(x, i, a.width);
-    if constexpr (ADD) {
-      v = add8<BF>(v, load8<VEC>(res, i, a.width));
-      store8<VEC>(res, i, a.width, v);
-    }
-    take8<BF, NORM>(v, NORM ? load8<VEC>(a.w, i, a.width) : make_uint4(0, 0, 0, 0), t, ss, top);
-  };
-  float t[NC ? NC : 1][8];
+  f2 t[NC ? NC : 1][4];
+  const uint4 none = make_uint4(0, 0, 0, 0);
   if constexpr (NC) {
+    uint4 v[NC], r[ADD ? NC : 1], w[NORM ? NC : 1];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const int i = threadIdx.x * 8 + c * step;
-      if (i < a.width) fetch(i, t[c]);
+      const Piece<VEC> pc(tid, c, n, a.width);
+      v[c] = pc.load(x);
+      if constexpr (ADD) r[c] = pc.load(res);
+      if constexpr (NORM) w[c] = pc.load(a.w);
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      if constexpr (ADD) {
+        v[c] = add8<BF>(v[c], r[c]);
+        Piece<VEC>(tid, c, n, a.width).store(res, v[c]);
+      }
+      take8<BF, NORM>(v[c], NORM ? w[NORM ? c : 0] : none, t[c], squares, most);
     }
   } else {
-    for (int i = threadIdx.x * 8; i < a.width; i += step) fetch(i, t[0]);
+    for (int c = 0; c * n * 8 < a.width; ++c) {
+      const Piece<VEC> pc(tid, c, n, a.width);
+      uint4 v = pc.load(x);
+      if constexpr (ADD) {
+        v = add8<BF>(v, pc.load(res));
+        pc.store(res, v);
+      }
+      take8<BF, NORM>(v, NORM ? pc.load(a.w) : none, t[0], squares, most);
+    }
   }
-  top = __reduce_max_sync(0xffffffffu, top);
-  if constexpr (NORM) ss = warp_sum(ss);
-  if (lane == 0) {
-    red_top[warp] = top;
-    red_ss[warp] = ss;
+  float ss = 0.f;
+  if constexpr (NORM) {
+    float lo, hi;
+    unpack2(squares, lo, hi);
+    ss = warp_sum(lo + hi);
   }
-  __syncthreads();
-  const int warps = blockDim.x >> 5;
-  ss = 0.f;
-  for (int i = 0; i < warps; ++i) {
-    top = max(top, red_top[i]);
-    if constexpr (NORM) ss += red_ss[i];
+  uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
+  if constexpr (!WARP) {
+    if (lane == 0) {
+      red_top[warp] = top;
+      red_ss[warp] = ss;
+    }
+    __syncthreads();
+    const int warps = blockDim.x >> 5;
+    top = __reduce_max_sync(0xffffffffu, lane < warps ? red_top[lane] : 0u);
+    if (NORM && warp == 0) ss = warp_sum(lane < warps ? red_ss[lane] : 0.f);
   }
   const bool finite = top < 0x7f800000u;
   const float A = __uint_as_float(top);
-  if (threadIdx.x == 0) {
+  if (tid == 0) {
     float s = A;
     if constexpr (NORM) s *= rsqrtf(ss / static_cast<float>(a.width) + a.eps);
-    a.scales[blockIdx.x] = finite ? s / 127.f : __uint_as_float(0x7fc00000u);
+    a.scales[row] = finite ? s / 127.f : __uint_as_float(0x7fc00000u);
   }
-  const Coder code(finite ? A : 0.f);
-  auto put = [&](int i, const float (&v)[8]) {
-    uint32_t q[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) q[j] = finite ? code(v[j]) : 0u;
-    store8<VEC>(out, i, a.width, low_bytes(q[0], q[1], q[2], q[3]), low_bytes(q[4], q[5], q[6], q[7]));
-  };
+  const Coder<BF || !NORM> code(finite ? A : 0.f);
   if constexpr (NC) {
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      const int i = threadIdx.x * 8 + c * step;
-      if (i < a.width) put(i, t[c]);
-    }
+    for (int c = 0; c < NC; ++c) Piece<VEC>(tid, c, n, a.width).store(out, finite ? code(t[c]) : make_uint2(0, 0));
   } else {
-    for (int i = threadIdx.x * 8; i < a.width; i += step) {
-      const uint4 v = ADD ? load8<VEC>(res, i, a.width) : load8<VEC>(x, i, a.width);
-      take8<BF, NORM>(v, NORM ? load8<VEC>(a.w, i, a.width) : make_uint4(0, 0, 0, 0), t[0], ss, top);
-      put(i, t[0]);
+    for (int c = 0; c * n * 8 < a.width; ++c) {
+      const Piece<VEC> pc(tid, c, n, a.width);
+      take8<BF, NORM>(pc.load(ADD ? res : x), NORM ? pc.load(a.w) : none, t[0], squares, most);
+      pc.store(out, finite ? code(t[0]) : make_uint2(0, 0));
     }
   }
 }
 
+// How a row is shared, measured as device time of calls that follow each other (us):
+//   a warp per row   16 384 rows of 64 - 1 024 to codes: 3.8 - 8.7, a block per row 17.9 (1.1 ns a block, whatever it does); with the
+//                    residual up to 512 wide: 13.7 and 17.9, but 1 024 wide 20.6 and 18.3.  Below 1 000 rows there is nothing in it.
+//   pieces a thread  many rows: to codes, 8 192 x 14 336 with 8 / 4 pieces 57 / 66, x 4 096 with 4 / 2 30.5 / 32.7; with the residual,
+//                    whose loads are twice as many, 8 192 x 8 192 with 2 / 4 69.3 / 70.9.  Few rows: as many threads as there are.
+// Rows that do not lie on 16 bytes take more instructions than the loads hide: 2 pieces, or the loop (8 192 x 16 383: 141).
 template <bool BF, bool NORM, bool ADD, bool VEC>
 static void launch(const Args& a, cudaStream_t st) {
-  const int pieces = (a.width + 7) / 8;
-  const auto go = [&](auto kern, int nc) {
-    const int threads = nc ? ((pieces + nc - 1) / nc + 31) / 32 * 32 : 1024;
-    launch_pdl(kern, dim3(a.rows), dim3(threads), 0, st, a);
+  const int pieces = (a.width - 1) / 8 + 1;
+  const auto go = [&](auto kern, int blocks, int threads) {
+    launch_pdl(kern, dim3(blocks), dim3(threads), 0, st, a);
     B200_CUDA_LAUNCH_CHECK();
   };
-  if (pieces <= 256) go(rows_i8_kernel<BF, NORM, ADD, VEC, 1>, 1);
-  else if (pieces <= 1024) go(rows_i8_kernel<BF, NORM, ADD, VEC, 2>, 2);
-  else if (pieces <= 4096) go(rows_i8_kernel<BF, NORM, ADD, VEC, 4>, 4);
-  else go(rows_i8_kernel<BF, NORM, ADD, VEC, 0>, 0);
+  if (a.rows >= 1000 && pieces <= (ADD ? 64 : 128)) {
+    const int blocks = (a.rows - 1) / kWarpRows + 1;
+    if (pieces <= 32) go(rows_i8_kernel<BF, NORM, ADD, VEC, true, 1>, blocks, 32 * kWarpRows);
+    else go(rows_i8_kernel<BF, NORM, ADD, VEC, true, 4>, blocks, 32 * kWarpRows);
+    return;
+  }
+  const bool many = a.rows > 2 * sm_count();
+  const int most = !many || ADD || !VEC ? 512 : NORM ? 256 : 128;      // threads
+  int nc = many && ADD ? 2 : 1;
+  while (nc < 8 && pieces > nc * most) nc *= 2;
+  const auto threads = [&] { return ((pieces - 1) / nc / 32 + 1) * 32; };
+  if (pieces > 512 * nc || (!VEC && nc > 2)) return go(rows_i8_kernel<BF, NORM, ADD, VEC, false, 0>, a.rows, 1024);
+  if (nc == 1) return go(rows_i8_kernel<BF, NORM, ADD, VEC, false, 1>, a.rows, threads());
+  if (nc == 2) return go(rows_i8_kernel<BF, NORM, ADD, VEC, false, 2>, a.rows, threads());
+  if constexpr (VEC) {
+    if (nc == 4) return go(rows_i8_kernel<BF, NORM, ADD, VEC, false, 4>, a.rows, threads());
+    go(rows_i8_kernel<BF, NORM, ADD, VEC, false, 8>, a.rows, threads());
+  }
 }
 
 template <bool BF, bool NORM, bool ADD>
@@ -228,21 +367,21 @@ static void rows_i8(void* out, float* scales, void* residual, const void* x, con
                                            int32_t hidden, float eps, int64_t stream) {                                        \
     using namespace b200;                                                                                                      \
     if (num_tokens <= 0) return;                                                                                               \
-    B200_CHECK_ARG(out && scales && x && weight && hidden > 0, "rmsnorm_i8: bad arguments");                                   \
+    B200_CHECK_ARG(out && scales && x && weight && hidden > 0 && hidden <= rows8::kMaxWidth, "rmsnorm_i8: bad arguments");     \
     rows8::rows_i8<BF, true, false>(out, scales, nullptr, x, weight, num_tokens, hidden, eps, stream);                         \
   }                                                                                                                            \
   extern "C" void b200_add_rmsnorm_i8_##SUFFIX(void* out, float* scales, void* residual, const void* x, const void* weight,    \
                                                int32_t num_tokens, int32_t hidden, float eps, int64_t stream) {                \
     using namespace b200;                                                                                                      \
     if (num_tokens <= 0) return;                                                                                               \
-    B200_CHECK_ARG(out && scales && residual && x && weight && hidden > 0, "add_rmsnorm_i8: bad arguments");                   \
+    B200_CHECK_ARG(out && scales && residual && x && weight && hidden > 0 && hidden <= rows8::kMaxWidth, "add_rmsnorm_i8: bad arguments");\
     rows8::rows_i8<BF, true, true>(out, scales, residual, x, weight, num_tokens, hidden, eps, stream);                         \
   }                                                                                                                            \
   extern "C" void b200_quant_rows_i8_##SUFFIX(void* out, float* scales, const void* x, int32_t rows, int32_t width,            \
                                               int64_t stream) {                                                                \
     using namespace b200;                                                                                                      \
     if (rows <= 0) return;                                                                                                     \
-    B200_CHECK_ARG(out && scales && x && width > 0, "quant_rows_i8: bad arguments");                                           \
+    B200_CHECK_ARG(out && scales && x && width > 0 && width <= rows8::kMaxWidth, "quant_rows_i8: bad arguments");              \
     rows8::rows_i8<BF, false, false>(out, scales, nullptr, x, nullptr, rows, width, 0.f, stream);                              \
   }
 B200_ROWS_I8(f16, false)

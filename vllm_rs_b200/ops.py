@@ -116,89 +116,111 @@ def wna16_dequant(w_packed, scales, qzeros, *, k: int, n: int, bits=4, group_siz
 
 
 # ------------------------------------------------------------------ linear layers in 8-bit integers
-def _i8_rows(x, w, residual, out, scales):
-    """Checks of what becomes int8 rows; the output's and the scales' tensors."""
-    _cuda(x, w, residual, out, scales)
-    if x.dim() != 2:
-        raise ValueError(f"rows must be [rows, width], got {tuple(x.shape)}")
-    rows, width = x.shape
-    for t, shape, what in ((w, (width,), "weight"), (residual, (rows, width), "residual")):
-        if t is not None and (t.shape != shape or t.dtype != x.dtype):
-            raise ValueError(f"{what} must be {shape} in {x.dtype}, got {tuple(t.shape)} in {t.dtype}")
-    if out is None:
-        out = torch.empty(rows, width, dtype=torch.int8, device=x.device)
-    elif out.shape != (rows, width) or out.dtype != torch.int8:
-        raise ValueError(f"out must be {(rows, width)} in int8, got {tuple(out.shape)} in {out.dtype}")
-    if scales is None:
-        scales = torch.empty(rows, dtype=torch.float32, device=x.device)
-    elif scales.shape != (rows,) or scales.dtype != torch.float32:
-        raise ValueError(f"scales must be {(rows,)} in float32, got {tuple(scales.shape)} in {scales.dtype}")
-    _here(x, w, residual, out, scales)
-    return rows, width, out, scales
+# Small calls cost what the host does: entry points are looked up once, every tensor is asked twice at most.
+_i8_entries = {}
 
 
-def _here(*ts):
-    """Kernels go to the current device's stream: what they read and write has to be there."""
+def _i8_entry(stem: str, dtype):
+    """The flavour of an entry point that `dtype` (16 bits; results of products also float32) names."""
+    fn = _i8_entries.get((stem, dtype))
+    if fn is None:
+        names = {torch.float16: "_f16", torch.bfloat16: "_bf16"}
+        if stem == "b200_gemm_i8":
+            names[torch.float32] = "_f32"
+        if dtype not in names:
+            raise TypeError(f"{stem}: {dtype} is none of {', '.join(map(str, names))}")
+        fn = _i8_entries[stem, dtype] = getattr(_lib.lib(), stem + names[dtype])
+    return fn
+
+
+def _on_device(*ts):
+    """Kernels go to the current device's stream: what they read and write lies there, without gaps."""
     dev = torch.cuda.current_device()
     for t in ts:
-        if t is not None and t.get_device() != dev:
-            raise ValueError(f"a tensor lies on cuda:{t.get_device()}, the current device is cuda:{dev}")
+        if t is not None and not (t.get_device() == dev and t.is_contiguous()):
+            raise ValueError(f"b200 ops need contiguous CUDA tensors of the current device, cuda:{dev}; got one on {t.device} with "
+                             f"strides {t.stride()}")
+
+
+def _expect(t, shape, dtype, what):
+    if t.dtype != dtype or t.shape != shape:
+        raise ValueError(f"{what} must be {shape} in {dtype}, got {tuple(t.shape)} in {t.dtype}")
+
+
+def _i8_rows(x, out, scales, w=None, residual=None):
+    """Checks of what becomes int8 rows; rows, width, and the tensors of the codes and scales."""
+    if x.dim() != 2:
+        raise ValueError(f"rows must be [rows, width], got {tuple(x.shape)}")
+    shape = rows, width = x.shape
+    if w is not None:
+        _expect(w, (width,), x.dtype, "weight")
+    if residual is not None:
+        _expect(residual, shape, x.dtype, "residual")
+    if out is not None:
+        _expect(out, shape, torch.int8, "out")
+    if scales is not None:
+        _expect(scales, (rows,), torch.float32, "scales")
+    _on_device(x, w, residual, out, scales)
+    if out is None:
+        out = torch.empty_like(x, dtype=torch.int8)
+    if scales is None:
+        scales = torch.empty(rows, dtype=torch.float32, device=x.device)
+    return rows, width, out, scales
 
 
 def quant_rows_i8(x, out=None, scales=None):
     """Rows [R, W] (fp16 / bf16) to int8 codes and a scale per row (fp32): value = code * scale, codes = round(127 x / max|x|), ties
     to even, exactly.  Activations before an int8 product, and weights [N, K] when they are loaded.  Returns (codes, scales)."""
-    rows, width, out, scales = _i8_rows(x, None, None, out, scales)
-    _sym("b200_quant_rows_i8", x)(_p(out), _p(scales), _p(x), rows, width, _stream())
+    fn = _i8_entry("b200_quant_rows_i8", x.dtype)
+    rows, width, out, scales = _i8_rows(x, out, scales)
+    fn(out.data_ptr(), scales.data_ptr(), x.data_ptr(), rows, width, _stream())
     _lib.check()
     return out, scales
 
 
 def rmsnorm_i8(x, w, eps, out=None, scales=None):
     """rmsnorm(x) * w as int8 codes and a scale per token, without a 16-bit rounding between.  Returns (codes, scales)."""
-    rows, width, out, scales = _i8_rows(x, w, None, out, scales)
-    _sym("b200_rmsnorm_i8", x)(_p(out), _p(scales), _p(x), _p(w), rows, width, eps, _stream())
+    fn = _i8_entry("b200_rmsnorm_i8", x.dtype)
+    rows, width, out, scales = _i8_rows(x, out, scales, w)
+    fn(out.data_ptr(), scales.data_ptr(), x.data_ptr(), w.data_ptr(), rows, width, eps, _stream())
     _lib.check()
     return out, scales
 
 
 def add_rmsnorm_i8(residual, x, w, eps, out=None, scales=None):
     """residual += x (in place); rmsnorm(residual) * w as int8 codes and a scale per token.  Returns (codes, scales)."""
-    rows, width, out, scales = _i8_rows(x, w, residual, out, scales)
-    _sym("b200_add_rmsnorm_i8", x)(_p(out), _p(scales), _p(residual), _p(x), _p(w), rows, width, eps, _stream())
+    fn = _i8_entry("b200_add_rmsnorm_i8", x.dtype)
+    rows, width, out, scales = _i8_rows(x, out, scales, w, residual)
+    fn(out.data_ptr(), scales.data_ptr(), residual.data_ptr(), x.data_ptr(), w.data_ptr(), rows, width, eps, _stream())
     _lib.check()
     return out, scales
-
-
-_GEMM_I8 = {torch.float16: "b200_gemm_i8_f16", torch.bfloat16: "b200_gemm_i8_bf16", torch.float32: "b200_gemm_i8_f32"}
 
 
 def gemm_i8(x, x_scales, w_nk, w_scales, bias=None, epilogue=EPI_NONE, dtype=torch.float16, out=None):
     """int8 rows [M, K] times int8 weights [N, K], scales fp32 per row and per output channel, optional bias [N] in the output's
     type: y = (x @ w^T) * x_scales * w_scales + bias, exact int32 sums, one rounding.  EPI_SILU_MUL: weights [gate | up],
     y [M, N / 2] = silu(gate) * up.  K is a multiple of 16.  `dtype`: of the output, float16, bfloat16 or float32."""
-    _cuda(x, x_scales, w_nk, w_scales, bias, out)
-    if x.dim() != 2 or w_nk.dim() != 2 or x.dtype != torch.int8 or w_nk.dtype != torch.int8 or x.shape[1] != w_nk.shape[1]:
-        raise ValueError(f"int8 rows [M, K] and weights [N, K] are needed, got {tuple(x.shape)} in {x.dtype} and "
-                         f"{tuple(w_nk.shape)} in {w_nk.dtype}")
+    fn = _i8_entry("b200_gemm_i8", dtype)
+    if x.dim() != 2 or w_nk.dim() != 2:
+        raise ValueError(f"rows [M, K] and weights [N, K] are needed, got {tuple(x.shape)} and {tuple(w_nk.shape)}")
     (m, k), n = x.shape, w_nk.shape[0]
-    if x_scales.shape != (m,) or w_scales.shape != (n,) or x_scales.dtype != torch.float32 or w_scales.dtype != torch.float32:
-        raise ValueError(f"scales must be float32, {(m,)} and {(n,)}, got {tuple(x_scales.shape)} in {x_scales.dtype} and "
-                         f"{tuple(w_scales.shape)} in {w_scales.dtype}")
-    if dtype not in _GEMM_I8:
-        raise TypeError(f"gemm_i8: results are float16, bfloat16 or float32, not {dtype}")
-    if bias is not None and (bias.shape != (n,) or bias.dtype != dtype):
-        raise ValueError(f"bias must be {(n,)} in {dtype}, got {tuple(bias.shape)} in {bias.dtype}")
-    if epilogue not in (EPI_NONE, EPI_SILU_MUL) or (epilogue == EPI_SILU_MUL and n % 2):
-        raise ValueError(f"gemm_i8: epilogue {epilogue} with {n} weight rows")
-    cols = n // 2 if epilogue == EPI_SILU_MUL else n
+    _expect(x, (m, k), torch.int8, "rows")
+    _expect(w_nk, (n, k), torch.int8, "weights")
+    _expect(x_scales, (m,), torch.float32, "rows' scales")
+    _expect(w_scales, (n,), torch.float32, "weights' scales")
+    if bias is not None:
+        _expect(bias, (n,), dtype, "bias")
+    cols = n
+    if epilogue != EPI_NONE:
+        if epilogue != EPI_SILU_MUL or n % 2:
+            raise ValueError(f"gemm_i8: epilogue {epilogue} with {n} weight rows")
+        cols = n // 2
+    if out is not None:
+        _expect(out, (m, cols), dtype, "out")
+    _on_device(x, x_scales, w_nk, w_scales, bias, out)
     if out is None:
-        out = torch.empty(m, cols, dtype=dtype, device=x.device)
-    elif out.shape != (m, cols) or out.dtype != dtype:
-        raise ValueError(f"out must be {(m, cols)} in {dtype}, got {tuple(out.shape)} in {out.dtype}")
-    _here(x, x_scales, w_nk, w_scales, bias, out)
-    getattr(_lib.lib(), _GEMM_I8[dtype])(_p(x), _p(x_scales), _p(w_nk), _p(w_scales), _p(bias), _p(out), m, n, k, epilogue,
-                                         _stream())
+        out = torch.empty((m, cols), dtype=dtype, device=x.device)
+    fn(x.data_ptr(), x_scales.data_ptr(), w_nk.data_ptr(), w_scales.data_ptr(), _p(bias), out.data_ptr(), m, n, k, epilogue, _stream())
     _lib.check()
     return out
 
