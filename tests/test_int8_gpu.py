@@ -169,8 +169,8 @@ def _check_product(y, a, sa, w, sw, bias, dtype, silu=False):
         g, u, dg, du = v[:, :n], v[:, n:], off[:, :n], off[:, n:]
         sig = torch.sigmoid(g)
         want = g * sig * u
-        # |silu'| <= 1.1; exponential (2 steps of 2^-23), sum, division, product
-        off = 1.1 * dg * u.abs() + (g * sig).abs() * du + 1.1 * dg * du + 7 * U * want.abs()
+        # |silu'| <= 1.1; exponential (2 steps of 2^-23), 1 + e, its reciprocal, three products
+        off = 1.1 * dg * u.abs() + (g * sig).abs() * du + 1.1 * dg * du + 9 * U * want.abs()
     else:
         want = v
     half = torch.finfo(dtype).eps / 2

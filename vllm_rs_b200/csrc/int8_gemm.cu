@@ -2,14 +2,25 @@
 //   y[m, n] = (sum_k a[m, k] w[n, k]) * a_scales[m] * w_scales[n] (+ bias[n])      int32 sums, exact up to K = 131056
 // rounded once to fp16, bf16 or fp32.  SiLU: w holds gate rows, then as many up rows; out[m, n] = silu(gate) * up of the fp32 values.
 //
-// Tiles of 64 x 64 from shared memory, four products per dp4a.
+// Three forms, all with the same arithmetic behind the exact sums, so that a result does not depend on which one ran (`launch` and
+// `plan` choose, with what was measured there):
+//   gemv_kernel    one row or two: dp4a, weights straight to registers.  Bound: HBM, and the launch's start and end.
+//   split_kernel   up to some thousand rows: one tile per block or pair of blocks, K shared by the blocks of a cluster.  Bound: HBM up to
+//                  some 100 rows (32 x 28 672 x 4 096 gated 21.6 us, floor 18.2; x 128 256 85.9 and 82.9), then what the L2
+//                  delivers to the SMs (257 x 4 096 x 14 336: 21.6 us, HBM alone 9.9).
+//   pair_kernel    many rows: persistent pairs of blocks.  Bound: the tensor cores, in long runs under the power cap (8 192 x 28 672 x
+//                  4 096 gated: 2.9 - 3.1 PFLOP/s; cuBLAS in bf16 reaches 1.64 in a burst, 1.37 sustained).
 #include "../../include/b200_vllm.h"
+#include <algorithm>
 #include "common.cuh"
+#include "host/per_device.hpp"
 
 namespace b200 {
 namespace gemm8 {
 
 constexpr int kMaxK = 131056;        // 2^31 / 128^2 = 131072 products of the largest size overflow; the multiple of 16 below
+constexpr int kBK = 128;             // K of a stage: one 128-byte swizzle row, four products of 32
+constexpr uint32_t kHiSw128 = (1024 >> 4) | (1u << 14) | (2u << 29);
 
 enum Out { kF16 = 0, kBF16 = 1, kF32 = 2 };
 
@@ -23,6 +34,47 @@ struct Args {
   int M, N, K;
 };
 
+// Instruction descriptor, kind::i8: int32 sums (bits [4,6) = 2), signed A and B ([7,10) = [10,13) = 1), both K-major, no saturation.
+__host__ __device__ constexpr uint32_t make_idesc_i8(int M, int N) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(N >> 3) << 17) | (uint32_t(M >> 4) << 24);
+}
+
+template <int CG>
+__device__ __forceinline__ void mma_i8(uint32_t lead, uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
+  if constexpr (CG == 1)
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t"
+        "setp.ne.b32 q, %0, 0;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "mov.b64 da, {%2, %5};\n\tmov.b64 db, {%3, %5};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::i8 [%1], da, db, %4, p;\n\t}\n" ::"r"(lead),
+        "r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(kHiSw128), "r"(acc)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t"
+        "setp.ne.b32 q, %0, 0;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "mov.b64 da, {%2, %5};\n\tmov.b64 db, {%3, %5};\n\t"
+        "@q tcgen05.mma.cta_group::2.kind::i8 [%1], da, db, %4, p;\n\t}\n" ::"r"(lead),
+        "r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(kHiSw128), "r"(acc)
+        : "memory");
+}
+// on this barrier in the blocks of `mask` (one block: its own)
+template <int CG>
+__device__ __forceinline__ void commit(uint32_t lead, uint64_t* bar, uint16_t mask = 3) {
+  if constexpr (CG == 1)
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %0, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%1];\n\t}\n" ::"r"(lead),
+        "r"(smem_u32(bar))
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %0, 0;\n\t"
+        "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%1], %2;\n\t}\n" ::"r"(lead),
+        "r"(smem_u32(bar)), "h"(mask)
+        : "memory");
+}
+
 template <int OUT>
 __device__ __forceinline__ float load_elem(const void* p, size_t i) {
   if constexpr (OUT == kF32) return static_cast<const float*>(p)[i];
@@ -33,48 +85,742 @@ __device__ __forceinline__ void store_elem(void* p, size_t i, float v) {
   if constexpr (OUT == kF32) static_cast<float*>(p)[i] = v;
   else static_cast<uint16_t*>(p)[i] = f32_to_bits16<OUT == kBF16>(v);
 }
-__device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.f + expf(-g)) * u; }
+// The epilogue's arithmetic, the same operations in every kernel: results do not depend on which one ran.
+__device__ __forceinline__ float scaled(int acc, float sa, float sw) { return __fmul_rn(__fmul_rn(static_cast<float>(acc), sa), sw); }
+// g / (1 + e^-g) u without a branch: with e = e^-|g| the denominator d lies in [1, 2], where the approximate reciprocal and one Newton
+// step are within a step of 1 / d.  (A division's slow path keeps four of them from overlapping: 0.6 us of a 32-token gate | up.)
+__device__ __forceinline__ float silu_mul(float g, float u) {
+  const float e = expf(-fabsf(g)), d = __fadd_rn(1.f, e);
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(d));
+  r = fmaf(r, fmaf(-d, r, 1.f), r);
+  return __fmul_rn(__fmul_rn(g < 0.f ? __fmul_rn(g, e) : g, r), u);
+}
+
+// ------------------------------------------------------------------ many rows
+// Persistent pairs of blocks walk tiles of 256 rows x bn weight rows (of a gated tile half are gate rows and half the up rows of the
+// same channels).  Each block stages its 128 rows and half of the weight rows; the first one issues the pair's products.
+// Warp 0 copies, warp 1 multiplies into one of two accumulators, warps 2-9 scale and store under the next tile's products.
+// After a wait has given up (*fail) all others return at once and the loops run out.
+constexpr int kPairThreads = 320, kEpiWarps = 8, kPairStages = 6, kPairStage = 2 * 128 * 128;
+constexpr int kPitch = 80, kOutBytes = kEpiWarps * 32 * kPitch;      // a warp's 32 rows x 64 bytes on their way out
+constexpr int kPairScales = kPairStages * kPairStage + kOutBytes;    // [2][256] scales, [2][256] bias
+constexpr int kPairBars = kPairScales + 4 * 256 * 4;
+constexpr int kPairSmem = kPairBars + (2 * kPairStages + 5) * 8 + 16 + 1024;
+static_assert(kPairSmem <= 227 * 1024, "shared memory budget");
+
+struct PairArgs {
+  Args g;
+  int n_out, KB, bn, tiles_m, tiles_n, group_m, wide;
+  int* err;
+};
 
 template <int OUT, bool SILU>
-__global__ void __launch_bounds__(256) simple_kernel(const Args g) {
-  __shared__ int sa[64][17], sw[SILU ? 2 : 1][64][17];
+__global__ void __launch_bounds__(kPairThreads, 1)
+pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap wmap, const PairArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* scale_of = reinterpret_cast<float*>(smem + kPairScales);    // [2][256]
+  float* bias_of = scale_of + 2 * 256;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kPairBars);
+  uint64_t* empty = full + kPairStages;
+  uint64_t* tfull = empty + kPairStages;           // [2] accumulator complete
+  uint64_t* tempty = tfull + 2;                    // [2] accumulator read
+  uint64_t* drained = tempty + 2;
+  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(drained + 1);
+  volatile int* fail = reinterpret_cast<volatile int*>(tmem_ptr + 1);
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(cluster_ctarank()), unit = blockIdx.x >> 1, units = gridDim.x >> 1;
+  const int ntiles = a.tiles_m * a.tiles_n, cols = SILU ? a.bn / 2 : a.bn;
+
   pdl_trigger();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kPairStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int s = 0; s < 2; ++s) { mbar_init(&tfull[s], 1); mbar_init(&tempty[s], kEpiWarps * 2); }
+    mbar_init(drained, 1);
+    *fail = 0;
+    fence_barrier_init();
+    prefetch_tmap(&amap);
+    prefetch_tmap(&wmap);
+  }
+  if (warp == 1) {
+    tmem_alloc_cg2(tmem_ptr, 512);
+    tmem_relinquish_cg2();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_arrive();                                // the other block's barriers are there
+  cluster_wait();
+  tc_fence_after();
   pdl_wait();
-  const int n_out = SILU ? g.N / 2 : g.N, m0 = blockIdx.y * 64, n0 = blockIdx.x * 64;
-  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15, kw = g.K / 4;
-  int acc[SILU ? 2 : 1][4][4] = {};
-  for (int k0 = 0; k0 < kw; k0 += 16) {
-    for (int i = threadIdx.x; i < 64 * 16; i += 256) {
-      const int r = i >> 4, k = i & 15;
-      const bool in = k0 + k < kw;
-      sa[r][k] = in && m0 + r < g.M ? reinterpret_cast<const int*>(g.a)[static_cast<size_t>(m0 + r) * kw + k0 + k] : 0;
-#pragma unroll
-      for (int h = 0; h < (SILU ? 2 : 1); ++h)
-        sw[h][r][k] = in && n0 + r < n_out ? reinterpret_cast<const int*>(g.w)[static_cast<size_t>(h * n_out + n0 + r) * kw + k0 + k] : 0;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_ptr, 0);
+  // group_m row tiles, then the next weight tile: their rows stay in L2 while the weights pass once per group
+  auto tile_at = [&](int t, int& tm, int& tn) {
+    const int per = a.group_m * a.tiles_n, g = t / per, r = t - g * per, rows = min(a.group_m, a.tiles_m - g * a.group_m);
+    tn = r / rows;
+    tm = g * a.group_m + (r - tn * rows);
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ operands
+    int s = 0, armed = 0;
+    uint32_t ph = 0;
+    bool free_ = true;
+    const uint32_t bytes = 2 * 128 * kBK + a.bn * kBK;               // of the pair
+    for (int t = unit; t < ntiles && free_; t += units) {
+      int tm, tn;
+      tile_at(t, tm, tn);
+      const int arow = (tm * 2 + rank) * 128, wrow = SILU ? rank * a.n_out + tn * cols : tn * a.bn + rank * (a.bn / 2);
+      for (int kb = 0; kb < a.KB; ++kb) {
+        free_ = __all_sync(0xffffffffu, mbar_wait_limited(&empty[s], ph ^ 1, fail, a.err));
+        if (!free_) break;                         // a stage that did not come free is not armed again
+        uint8_t* dst = smem + s * kPairStage;
+        if (elect_one()) {                         // both blocks' bytes count on the first one's barrier
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], bytes);
+          const uint32_t bar = mapa_shared(smem_u32(&full[s]), 0);
+          tma_load_2d_cg2(dst, &amap, bar, kb * kBK, arow);
+          tma_load_2d_cg2(dst + 128 * kBK, &wmap, bar, kb * kBK, wrow);
+        }
+        ++armed;
+        if (++s == kPairStages) { s = 0; ph ^= 1; }
+      }
     }
-    __syncthreads();
+    if (lane == 0 && rank == 0 && *fail)           // copies in flight land before the block ends (the second waits for the first)
+      for (int i = 0; i < kPairStages && i < armed; ++i)
+        mbar_wait_limited(&full[i], ((armed - 1 - i) / kPairStages) & 1, nullptr, a.err);
+    __syncwarp();
+  } else if (warp == 1 && rank == 0) {
+    // ------------------------------------------------------------ products
+    const uint32_t idesc = make_idesc_i8(256, a.bn), lead = elect_one() ? 1u : 0u;
+    const uint32_t base = (smem_u32(smem) >> 4) | (1u << 16);
+    int s = 0, it = 0;
+    uint32_t ph = 0;
+    for (int t = unit; t < ntiles; t += units, ++it) {
+      const int buf = it & 1;
+      mbar_wait_limited(&tempty[buf], ((it >> 1) & 1) ^ 1, fail, a.err);
+      tc_fence_after();
+      const uint32_t d = tmem + buf * 256;
+      for (int kb = 0; kb < a.KB; ++kb) {
+        mbar_wait_limited(&full[s], ph, fail, a.err);
+        tc_fence_after();
+        const uint32_t a_lo = base + s * (kPairStage >> 4), b_lo = a_lo + (128 * kBK >> 4);
 #pragma unroll
-    for (int k = 0; k < 16; ++k)
+        for (int ks = 0; ks < kBK / 32; ++ks) mma_i8<2>(lead, d, a_lo + ks * 2, b_lo + ks * 2, idesc, (kb | ks) ? 1u : 0u);
+        commit<2>(lead, &empty[s]);
+        if (++s == kPairStages) { s = 0; ph ^= 1; }
+      }
+      commit<2>(lead, &tfull[buf]);
+    }
+    if (*fail) {                                   // products in flight end before TMEM is given back
+      commit<2>(lead, drained, 1);
+      mbar_wait_limited(drained, 0, nullptr, a.err);
+    }
+    __syncwarp();
+  } else if (warp > 1) {
+    // ------------------------------------------------------------ scales and stores
+    // A warp reads its quarter of the rows, every other 32 columns; four lanes then write 64 bytes of a row.
+    constexpr int kElem = OUT == kF32 ? 4 : 2;
+    const int q4 = warp & 3, tid = threadIdx.x - 64;
+    const uint32_t lanes = static_cast<uint32_t>(q4 * 32) << 16;
+    uint8_t* stage = smem + kPairStages * kPairStage + (warp - 2) * 32 * kPitch;
+    int it = 0;
+    for (int t = unit; t < ntiles; t += units, ++it) {
+      int tm, tn;
+      tile_at(t, tm, tn);
+      const int buf = it & 1, n0 = tn * cols, row0 = (tm * 2 + rank) * 128 + q4 * 32, rows = a.g.M - row0;
+      if (tid < a.bn) {                            // this tile's scales and bias, in the accumulator's order
+        const int j = SILU && tid >= cols ? tid - cols : tid, n = n0 + j, at = SILU && tid >= cols ? a.n_out + n : n;
+        scale_of[buf * 256 + tid] = n < a.n_out ? a.g.w_scales[at] : 0.f;
+        if (a.g.bias) bias_of[buf * 256 + tid] = n < a.n_out ? load_elem<OUT>(a.g.bias, at) : 0.f;
+      }
+      const float sa = lane < rows ? a.g.a_scales[row0 + lane] : 0.f;
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      mbar_wait_limited(&tfull[buf], (it >> 1) & 1, fail, a.err);
+      __syncwarp();
+      tc_fence_after();
+      const uint32_t src = tmem + lanes + buf * 256;
+      // the staged rows' bytes: `count` columns from c on
+      auto store = [&](int c, int count) {
+        __syncwarp();
+        if (a.wide) {
+          const int sub = (lane & 3) * 16, col = n0 + c + sub / kElem;
+          if (col < a.n_out) {
 #pragma unroll
-      for (int h = 0; h < (SILU ? 2 : 1); ++h)
+            for (int i = 0; i < 4; ++i) {
+              const int rw = i * 8 + (lane >> 2);
+              if (rw < rows)
+                *reinterpret_cast<uint4*>(static_cast<uint8_t*>(a.g.c) + (static_cast<size_t>(row0 + rw) * a.n_out + col) * kElem) =
+                    *reinterpret_cast<const uint4*>(stage + rw * kPitch + sub);
+            }
+          }
+        } else if (lane < count && n0 + c + lane < a.n_out) {
+          for (int rw = 0; rw < 32 && rw < rows; ++rw) {
+            const size_t at = static_cast<size_t>(row0 + rw) * a.n_out + n0 + c + lane;
+            if constexpr (OUT == kF32) static_cast<float*>(a.g.c)[at] = *reinterpret_cast<const float*>(stage + rw * kPitch + lane * 4);
+            else static_cast<uint16_t*>(a.g.c)[at] = *reinterpret_cast<const uint16_t*>(stage + rw * kPitch + lane * 2);
+          }
+        }
+        __syncwarp();
+      };
+      if (rows > 0) {
+#pragma unroll 1
+        for (int c = warp < 6 ? 0 : 32; c < cols; c += 64) {
+          uint32_t v[32], u[SILU ? 32 : 1];
+          tmem_ld_x32(src + c, v);
+          if constexpr (SILU) tmem_ld_x32(src + cols + c, u);
+          tc_wait_ld();
+          auto finish = [&](uint32_t (&x)[32], int c0) {
+            const float4* sc = reinterpret_cast<const float4*>(scale_of + buf * 256 + c0);
+            const float4* bi = reinterpret_cast<const float4*>(bias_of + buf * 256 + c0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+            for (int j = 0; j < 8; ++j) {
+              const float4 s4 = sc[j];
+              float f[4] = {scaled(static_cast<int>(x[4 * j]), sa, s4.x), scaled(static_cast<int>(x[4 * j + 1]), sa, s4.y),
+                            scaled(static_cast<int>(x[4 * j + 2]), sa, s4.z), scaled(static_cast<int>(x[4 * j + 3]), sa, s4.w)};
+              if (a.g.bias) {
+                const float4 b4 = bi[j];
+                f[0] = __fadd_rn(f[0], b4.x);
+                f[1] = __fadd_rn(f[1], b4.y);
+                f[2] = __fadd_rn(f[2], b4.z);
+                f[3] = __fadd_rn(f[3], b4.w);
+              }
 #pragma unroll
-          for (int j = 0; j < 4; ++j) acc[h][i][j] = __dp4a(sa[ty + 16 * i][k], sw[h][tx + 16 * j][k], acc[h][i][j]);
+              for (int e = 0; e < 4; ++e) x[4 * j + e] = __float_as_uint(f[e]);
+            }
+          };
+          finish(v, c);
+          if constexpr (SILU) {
+            finish(u, cols + c);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(silu_mul(__uint_as_float(v[j]), __uint_as_float(u[j])));
+          }
+          if constexpr (OUT == kF32) {
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+#pragma unroll
+              for (int i = 0; i < 16; i += 4)
+                *reinterpret_cast<uint4*>(stage + lane * kPitch + i * 4) =
+                    make_uint4(v[hf * 16 + i], v[hf * 16 + i + 1], v[hf * 16 + i + 2], v[hf * 16 + i + 3]);
+              store(c + hf * 16, 16);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              uint32_t h[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) h[e] = pack16x2<OUT == kBF16>(__uint_as_float(v[i + 2 * e]), __uint_as_float(v[i + 2 * e + 1]));
+              *reinterpret_cast<uint4*>(stage + lane * kPitch + i * 2) = make_uint4(h[0], h[1], h[2], h[3]);
+            }
+            store(c, 32);
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        // (what the products overwrite has been read; a release at cluster scope would wait for the results' stores)
+        if (rank != 0)
+          asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(mapa_shared(smem_u32(&tempty[buf]), 0)) : "memory");
+        else
+          mbar_arrive(&tempty[buf]);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_arrive();                                // neither block goes while the other can reach its memory
+  cluster_wait();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_cg2(tmem, 512);
+  }
+}
+
+// ------------------------------------------------------------------ few rows
+// A tile is 128 CG weight rows (lanes of the accumulator; gated: of every block's 128, 64 are gate rows and 64 the up rows of the
+// same channels) by T rows of a (its columns, in one product or two of nb).  CG = 2: pairs of blocks, each with its own weight rows
+// and half of the rows of a in shared memory.  `splits` parts of a cluster share K evenly; their int32 sums, exact in any order, meet
+// in shared memory: every block writes its own there, then takes its share of the rows of a from all that have the same weight
+// rows, scales and stores.  No workspace, one launch.
+constexpr int kMaxSmem = 227 * 1024, kSplitThreads = 320, kMaxStages = 24, kMaxT = 384;
+constexpr int kSplitFixed = 1024 + 512 + kMaxT * 4;          // alignment; barriers; the tile's a_scales
+
+struct SplitArgs {
+  Args g;
+  int n_out, KB, T, nb, tiles_m, splits, stages, stage_bytes, bar_off, tmem_cols, wide;
+  int* err;
+};
+
+template <int V> struct Int { static constexpr int value = V; };
+
+__device__ __forceinline__ uint4 ld_cluster_v4(uint32_t addr) {
+  uint4 r;
+  asm volatile("ld.shared::cluster.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(addr) : "memory");
+  return r;
+}
+
+template <int OUT, bool SILU, int CG>
+__global__ void __launch_bounds__(kSplitThreads)
+split_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap amap, const SplitArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + a.bar_off);
+  uint64_t* empty = full + a.stages;
+  uint64_t* done = empty + a.stages;
+  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* fail = reinterpret_cast<volatile int*>(tmem_ptr + 1);
+  float* row_scale = reinterpret_cast<float*>(smem + a.bar_off + 512);       // [T]
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int S = a.splits, C = S * CG;              // blocks of the cluster
+  const int rank = C > 1 ? static_cast<int>(cluster_ctarank()) : 0, part = rank / CG, half = rank % CG, tile = blockIdx.x / C;
+  const int tn = tile / a.tiles_m, tm = tile - tn * a.tiles_m;
+  constexpr int kChan = SILU ? 64 : 128;           // output channels of a block
+  const int n0 = (tn * CG + half) * kChan, m0 = tm * a.T;
+  const int kb0 = part * a.KB / S, kb1 = (part + 1) * a.KB / S;
+
+  pdl_trigger();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < a.stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    mbar_init(done, 1);
+    *fail = 0;
+    fence_barrier_init();
+    prefetch_tmap(&amap);
+    prefetch_tmap(&wmap);
+  }
+  if (warp == 1) {
+    if constexpr (CG == 2) {
+      tmem_alloc_cg2(tmem_ptr, a.tmem_cols);
+      tmem_relinquish_cg2();
+    } else {
+      tmem_alloc(tmem_ptr, a.tmem_cols);
+      tmem_relinquish();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (CG == 2) {                         // the other block's barriers are there
+    cluster_arrive();
+    cluster_wait();
+  }
+  tc_fence_after();
+  pdl_wait();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_ptr, 0);
+
+  // a lane's four channels at the end; gated: half a warp per row of a, the same lane has gate and up
+  const int ch = SILU ? (lane & 15) * 4 : lane * 4, n = n0 + ch;
+  float sw[4], su[4], bw[4] = {}, bu[4] = {};
+  auto channel_scales = [&] {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool in = n + j < a.n_out;
+      sw[j] = in ? a.g.w_scales[n + j] : 0.f;
+      if (SILU) su[j] = in ? a.g.w_scales[a.n_out + n + j] : 0.f;
+      if (a.g.bias && in) {
+        bw[j] = load_elem<OUT>(a.g.bias, n + j);
+        if (SILU) bu[j] = load_elem<OUT>(a.g.bias, a.n_out + n + j);
+      }
+    }
+  };
+  if (warp == 0) {
+    // ------------------------------------------------------------ operands
+    int s = 0, armed = 0;
+    uint32_t ph = 0;
+    const uint32_t bytes = (128 * CG + a.T) * kBK;           // of the pair
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!__all_sync(0xffffffffu, mbar_wait_limited(&empty[s], ph ^ 1, fail, a.err))) break;
+      uint8_t* dst = smem + s * a.stage_bytes;
+      uint8_t* tok = dst + 128 * kBK;
+      if (elect_one()) {
+        if constexpr (CG == 2) {                   // both blocks' bytes count on the first one's barrier
+          if (half == 0) mbar_arrive_expect_tx(&full[s], bytes);
+          const uint32_t bar = mapa_shared(smem_u32(&full[s]), rank & ~1);
+          tma_load_2d_cg2(dst, &wmap, bar, kb * kBK, n0);
+          if (SILU) tma_load_2d_cg2(dst + 64 * kBK, &wmap, bar, kb * kBK, a.n_out + n0);
+          for (int i = 0; i < a.T; i += a.nb, tok += a.nb / 2 * kBK)
+            tma_load_2d_cg2(tok, &amap, bar, kb * kBK, m0 + i + half * (a.nb / 2));
+        } else {
+          mbar_arrive_expect_tx(&full[s], bytes);
+          tma_load_2d(dst, &wmap, &full[s], kb * kBK, n0);
+          if (SILU) tma_load_2d(dst + 64 * kBK, &wmap, &full[s], kb * kBK, a.n_out + n0);
+          for (int i = 0; i < a.T; i += a.nb, tok += a.nb * kBK) tma_load_2d(tok, &amap, &full[s], kb * kBK, m0 + i);
+        }
+      }
+      ++armed;
+      if (++s == a.stages) { s = 0; ph ^= 1; }
+    }
+    if (lane == 0 && half == 0 && *fail)           // copies in flight land before the block ends (a pair's second waits for its first)
+      for (int i = 0; i < a.stages && i < armed; ++i)
+        mbar_wait_limited(&full[i], ((armed - 1 - i) / a.stages) & 1, nullptr, a.err);
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ products
+    if (half == 0) {
+      const uint32_t idesc = make_idesc_i8(128 * CG, a.nb), lead = elect_one() ? 1u : 0u;
+      const uint32_t base = (smem_u32(smem) >> 4) | (1u << 16);
+      const uint16_t mask = static_cast<uint16_t>(3u << (rank & ~1));
+      int s = 0;
+      uint32_t ph = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        mbar_wait_limited(&full[s], ph, fail, a.err);
+        tc_fence_after();
+        const uint32_t a_lo = base + s * (a.stage_bytes >> 4);
+        uint32_t b_lo = a_lo + (128 * kBK >> 4);
+        for (int i = 0; i < a.T; i += a.nb, b_lo += a.nb / CG * kBK >> 4)
+#pragma unroll
+          for (int ks = 0; ks < kBK / 32; ++ks) mma_i8<CG>(lead, tmem + i, a_lo + ks * 2, b_lo + ks * 2, idesc, (kb > kb0 || ks) ? 1u : 0u);
+        commit<CG>(lead, &empty[s], mask);
+        if (++s == a.stages) { s = 0; ph ^= 1; }
+      }
+      commit<CG>(lead, done, mask);
+      if (*fail) mbar_wait_limited(done, 0, nullptr, a.err);    // products in flight end before TMEM is given back
+      __syncwarp();
+    }
+  } else {
+    // this block's sums, [row of a][weight row], where the stages were: all of them have been read.  Two warps per quarter of the lanes.
+    for (int r = threadIdx.x - 64; r < a.T; r += kSplitThreads - 64) row_scale[r] = m0 + r < a.g.M ? a.g.a_scales[m0 + r] : 0.f;
+    channel_scales();
+    mbar_wait_limited(done, 0, fail, a.err);
+    __syncwarp();
+    tc_fence_after();
+    const int q4 = warp & 3;
+    uint32_t* sums = reinterpret_cast<uint32_t*>(smem) + q4 * 32 + lane;
+    for (int c = warp < 6 ? 0 : 32; c < a.T; c += 64) {
+      uint32_t v[32];
+      tmem_ld_x32(tmem + (static_cast<uint32_t>(q4 * 32) << 16) + c, v);
+      tc_wait_ld();
+#pragma unroll
+      for (int j = 0; j < 32; ++j) sums[(c + j) * 128] = v[j];
+    }
+  }
+  if (warp < 2) channel_scales();
+  tc_fence_before();
+  if (C > 1) {
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+  } else {
     __syncthreads();
   }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
-      if (m >= g.M || n >= n_out) continue;
-      float v[SILU ? 2 : 1];
+  constexpr int kPer = SILU ? 2 : 1, kStep = kSplitThreads / 32 * kPer;      // rows of a per warp at a time; of a turn
+  const int r0 = part * a.T / S, r1 = min((part + 1) * a.T / S, a.g.M - m0);
+  const uint32_t here = smem_u32(smem);
+  // kBatch turns at once, sums of kParts blocks at once
+  auto finish = [&](auto batch, auto parts) {
+    constexpr int kBatch = decltype(batch)::value, kParts = decltype(parts)::value;
+#pragma unroll 1
+    for (int rb = r0 + warp * kPer + (SILU ? lane >> 4 : 0); rb < r1; rb += kBatch * kStep) {
+      int x[kBatch][4] = {};
+      [[maybe_unused]] int y[SILU ? kBatch : 1][4] = {};
+      for (int p0 = 0; p0 < S; p0 += kParts) {       // asked for at once: another block's memory answers in 0.4 us
+        uint4 v[kParts][kBatch];
+        [[maybe_unused]] uint4 w[kParts][SILU ? kBatch : 1];
 #pragma unroll
-      for (int h = 0; h < (SILU ? 2 : 1); ++h) {
-        v[h] = static_cast<float>(acc[h][i][j]) * g.a_scales[m] * g.w_scales[h * n_out + n];
-        if (g.bias) v[h] += load_elem<OUT>(g.bias, h * n_out + n);
+        for (int q = 0; q < kParts; ++q) {
+          const uint32_t base = (C > 1 ? mapa_shared(here, min(p0 + q, S - 1) * CG + half) : here) + ch * 4;
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) {
+            const bool there = p0 + q < S && rb + i * kStep < r1;
+            v[q][i] = there ? ld_cluster_v4(base + (rb + i * kStep) * 512) : make_uint4(0, 0, 0, 0);
+            if constexpr (SILU) w[q][i] = there ? ld_cluster_v4(base + (rb + i * kStep) * 512 + 64 * 4) : make_uint4(0, 0, 0, 0);
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < kParts; ++q)
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) {
+            x[i][0] += static_cast<int>(v[q][i].x); x[i][1] += static_cast<int>(v[q][i].y);
+            x[i][2] += static_cast<int>(v[q][i].z); x[i][3] += static_cast<int>(v[q][i].w);
+            if constexpr (SILU) {
+              y[i][0] += static_cast<int>(w[q][i].x); y[i][1] += static_cast<int>(w[q][i].y);
+              y[i][2] += static_cast<int>(w[q][i].z); y[i][3] += static_cast<int>(w[q][i].w);
+            }
+          }
       }
-      store_elem<OUT>(g.c, static_cast<size_t>(m) * n_out + n, SILU ? silu_mul(v[0], v[SILU ? 1 : 0]) : v[0]);
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int r = rb + i * kStep;
+        if (r >= r1) break;
+        const float sa = row_scale[r];
+        float f[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          f[j] = scaled(x[i][j], sa, sw[j]);
+          if (a.g.bias) f[j] = __fadd_rn(f[j], bw[j]);
+          if constexpr (SILU) {
+            float u = scaled(y[i][j], sa, su[j]);
+            if (a.g.bias) u = __fadd_rn(u, bu[j]);
+            f[j] = silu_mul(f[j], u);
+          }
+        }
+        const size_t at = static_cast<size_t>(m0 + r) * a.n_out + n;
+        if (a.wide) {                                // four channels are all there or none
+          if (n < a.n_out) {
+            if constexpr (OUT == kF32) *reinterpret_cast<float4*>(static_cast<float*>(a.g.c) + at) = make_float4(f[0], f[1], f[2], f[3]);
+            else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.g.c) + at) =
+                make_uint2(pack16x2<OUT == kBF16>(f[0], f[1]), pack16x2<OUT == kBF16>(f[2], f[3]));
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (n + j < a.n_out) store_elem<OUT>(a.g.c, at + j, f[j]);
+        }
+      }
     }
+  };
+  if (S == 1) finish(Int<SILU ? 1 : 4>{}, Int<1>{});
+  else if (S == 2) finish(Int<SILU ? 2 : 8>{}, Int<2>{});
+  else finish(Int<SILU ? 1 : 4>{}, Int<4>{});
+  if (C > 1) {                                     // no block goes while another can read its sums; what it read is in use, the results
+    __syncwarp();                                  // that it stored need not have arrived (a release would wait for them: 0.7 us)
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    cluster_wait();
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    if constexpr (CG == 2) tmem_dealloc_cg2(tmem, a.tmem_cols);
+    else tmem_dealloc(tmem, a.tmem_cols);
+  }
+}
+
+// ------------------------------------------------------------------ one row to a few
+// A block has eight weight rows (gated: four gate rows and the up rows of the same channels); its warps take 512 of K in turn, eight
+// 16-byte loads a lane at once, four products per dp4a.
+constexpr int kGemvThreads = 256, kGemvRows = 8;
+
+template <int OUT, bool SILU, int MT>
+__global__ void __launch_bounds__(kGemvThreads, MT == 1 ? 4 : 3) gemv_kernel(const Args g, int n_out) {
+  constexpr int kChan = SILU ? kGemvRows / 2 : kGemvRows;
+  __shared__ int red[kGemvThreads / 32][kGemvRows * MT];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n0 = blockIdx.x * kChan;
+  const int8_t* w0 = g.w + static_cast<size_t>(n0) * g.K;
+  const size_t up = static_cast<size_t>(n_out) * g.K;
+  const int last = min(kChan, n_out - n0) - 1;     // (past the last channel: its row again)
+  const int8_t* a[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) a[m] = g.a + static_cast<size_t>(min(m, g.M - 1)) * g.K;
+  int acc[kGemvRows][MT] = {};
+  pdl_trigger();
+  pdl_wait();
+  for (int k = warp * 512 + lane * 16; k < g.K; k += kGemvThreads * 16) {
+    uint4 wv[kGemvRows], av[MT];
+#pragma unroll
+    for (int r = 0; r < kGemvRows; ++r) wv[r] = *reinterpret_cast<const uint4*>(w0 + (SILU && r >= kChan ? up : 0) + min(r % kChan, last) * g.K + k);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) av[m] = *reinterpret_cast<const uint4*>(a[m] + k);
+#pragma unroll
+    for (int r = 0; r < kGemvRows; ++r)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        int s = acc[r][m];
+        s = __dp4a(static_cast<int>(wv[r].x), static_cast<int>(av[m].x), s);
+        s = __dp4a(static_cast<int>(wv[r].y), static_cast<int>(av[m].y), s);
+        s = __dp4a(static_cast<int>(wv[r].z), static_cast<int>(av[m].z), s);
+        acc[r][m] = __dp4a(static_cast<int>(wv[r].w), static_cast<int>(av[m].w), s);
+      }
+  }
+#pragma unroll
+  for (int r = 0; r < kGemvRows; ++r)
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int s = __reduce_add_sync(0xffffffffu, acc[r][m]);
+      if (lane == 0) red[warp][m * kGemvRows + r] = s;
+    }
+  __syncthreads();
+  const int t = threadIdx.x, m = t / kChan, n = n0 + t % kChan;
+  if (t < kChan * MT && m < g.M && n < n_out) {
+    float v[2];
+#pragma unroll
+    for (int h = 0; h < (SILU ? 2 : 1); ++h) {
+      int s = 0;
+#pragma unroll
+      for (int i = 0; i < kGemvThreads / 32; ++i) s += red[i][m * kGemvRows + h * kChan + t % kChan];
+      v[h] = scaled(s, g.a_scales[m], g.w_scales[h * n_out + n]);
+      if (g.bias) v[h] = __fadd_rn(v[h], load_elem<OUT>(g.bias, h * n_out + n));
+    }
+    store_elem<OUT>(g.c, static_cast<size_t>(m) * n_out + n, SILU ? silu_mul(v[0], v[1]) : v[0]);
+  }
+}
+
+// ------------------------------------------------------------------ launches
+static bool map_rows(CUtensorMap* m, const void* base, int rows, int K, int box_rows) {
+  const uint64_t dims[2] = {static_cast<uint64_t>(K), static_cast<uint64_t>(rows)}, strides[1] = {static_cast<uint64_t>(K)};
+  const uint32_t box[2] = {kBK, static_cast<uint32_t>(box_rows)}, es[2] = {1, 1};
+  return encode_tensor_map(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, es,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B) == CUDA_SUCCESS;
+}
+template <typename K>
+static bool allow_smem(OncePerDevice& once, K kern, int bytes) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const cudaError_t e = once(dev, [&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); });
+  if (e != cudaSuccess) set_error(2, cudaGetErrorString(e));
+  return e == cudaSuccess;
+}
+
+template <int OUT, bool SILU>
+static void launch_pairs(const Args& g, int bn, cudaStream_t st) {
+  constexpr int kElem = OUT == kF32 ? 4 : 2;
+  PairArgs a;
+  a.g = g;
+  a.n_out = SILU ? g.N / 2 : g.N;
+  a.KB = (g.K + kBK - 1) / kBK;
+  a.bn = bn;
+  a.tiles_m = g.M / 256 + (g.M % 256 != 0);
+  a.tiles_n = (a.n_out + (SILU ? bn / 2 : bn) - 1) / (SILU ? bn / 2 : bn);
+  a.group_m = 16;
+  a.wide = ((reinterpret_cast<uintptr_t>(g.c) | (static_cast<uintptr_t>(a.n_out) * kElem)) & 15) == 0;
+  a.err = wait_error_flag();
+  CUtensorMap amap, wmap;
+  if (!map_rows(&amap, g.a, g.M, g.K, 128) || !map_rows(&wmap, g.w, g.N, g.K, bn / 2) || !a.err) {
+    set_error(2, "gemm_i8: cuTensorMapEncodeTiled failed");
+    return;
+  }
+  auto kern = pair_kernel<OUT, SILU>;
+  static OncePerDevice sized;
+  if (!allow_smem(sized, kern, kPairSmem)) return;
+  static const int most = [&] {
+    const int n = max_active_clusters(kern, dim3(sm_count() / 2 * 2), dim3(kPairThreads), kPairSmem, dim3(2));
+    return n > 0 ? n : sm_count() / 2;
+  }();
+  const int64_t tiles = static_cast<int64_t>(a.tiles_m) * a.tiles_n;
+  const int pairs = static_cast<int>(std::min<int64_t>(tiles, most));
+  const cudaError_t e = launch_pdl_cluster(kern, dim3(pairs * 2), dim3(kPairThreads), kPairSmem, st, dim3(2), amap, wmap, a);
+  if (e != cudaSuccess) set_error(2, cudaGetErrorString(e));
+  B200_CUDA_LAUNCH_CHECK();
+}
+
+template <int OUT, bool SILU, int MT>
+static void launch_gemv(const Args& g, cudaStream_t st) {
+  constexpr int kChan = SILU ? kGemvRows / 2 : kGemvRows;
+  const int n_out = SILU ? g.N / 2 : g.N;
+  launch_pdl(gemv_kernel<OUT, SILU, MT>, dim3((n_out - 1) / kChan + 1), dim3(kGemvThreads), 0, st, g, n_out);
+  B200_CUDA_LAUNCH_CHECK();
+}
+
+// Blocks of the split kernel that an SM holds take all of its shared memory or half of it.
+constexpr int kWholeSm = 226 * 1024, kHalfSm = 113 * 1024;
+
+// How many clusters of 1 to 8 of them the chip holds at once (of eight whole SMs: 15, since few groups of SMs have 16 to give).
+struct Room {
+  int whole[8], half[8];
+  Room() {
+    const auto kern = split_kernel<kF16, false, 1>;
+    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+    for (int c = 1; c <= 8; ++c) {
+      const dim3 grid(sm_count() / c * c);
+      const int w = max_active_clusters(kern, grid, dim3(kSplitThreads), kWholeSm, dim3(c));
+      const int h = max_active_clusters(kern, grid, dim3(kSplitThreads), kHalfSm, dim3(c));
+      whole[c - 1] = w > 0 ? w : sm_count() / c;
+      half[c - 1] = h > 0 ? h : 2 * sm_count() / c;
+    }
+  }
+};
+
+// What a product is cut into: `group` 0 pairs of blocks with tiles of 256 x T weight rows, 1 and 2 the split kernel with so many blocks
+// per tile and T rows of a.
+struct Plan {
+  int group, T, splits, smem;
+};
+
+// The estimates (us) are fits to 311 shapes (8 to 4 096 rows, N and K from 256 to 28 672), each measured in every form; the form taken
+// costs 1.5 % more than the best one in the mean, 20 % at most.  A block of K takes as long as the tensor core, the L2 (7.5 ns a
+// KB) or the memory's answer over the stages that wait for it; weights come at 7.2 TB/s at best; an epilogue 12 ns a row; a meeting
+// of parts 0.9 us and 0.27 for each further part.  What the choice is worth, us: 257 rows of 4 096 x 14 336 pairs 42, one part 28,
+// two parts 19.3, four of half an SM 24; 1 003 of 10 240 x 8 192 pairs 62.6 (256 wide 64.3), split 72.5.
+static Plan plan(const Args& g) {
+  static const Room room;
+  const int KB = (g.K + kBK - 1) / kBK;
+  const auto up = [](int x, int q) { return (x + q - 1) / q * q; };
+  Plan best{0, 256, 1, 0};
+  float least = 3.4e38f;
+  const auto offer = [&](float us, const Plan& p) {
+    if (us < least) {
+      least = us;
+      best = p;
+    }
+  };
+  if (g.M > 128)
+    for (int bn = 64; bn <= 256; bn += 64) {
+      const int64_t tiles = (static_cast<int64_t>(g.M) + 255) / 256 * ((g.N + bn - 1) / bn), pairs = sm_count() / 2;
+      const float block = std::max(bn * 0.58e-3f, (128 + bn / 2) * kBK * 9.04e-6f);
+      offer(2.75f + static_cast<float>((tiles + pairs - 1) / pairs) * (KB * block + 1.f) + bn * 5.96e-3f, Plan{0, bn, 1, 0});
+    }
+  if (g.M <= 1536)
+    for (int parts = 1; parts <= 5; ++parts) {
+      const int rows = (g.M + parts - 1) / parts;
+      if (rows <= kMaxT)
+        for (int group = 1; group <= 2; ++group) {
+          const int T = up(rows, rows > 256 || group == 2 ? 64 : 32);
+          const int64_t tiles = static_cast<int64_t>((g.N - 1) / (128 * group) + 1) * ((g.M + T - 1) / T);
+          const int stage = (128 + T / group) * kBK;
+          for (int splits = 1; splits * group <= 8 && splits <= KB; ++splits) {
+            const int c = splits * group - 1;
+            const bool whole = tiles <= room.whole[c];
+            if (!whole && T * 512 > kHalfSm - kSplitFixed) continue;
+            const int share = whole ? 1 : 2, smem = whole ? kWholeSm : kHalfSm;
+            const int64_t rounds = whole ? 1 : (tiles + room.half[c] - 1) / room.half[c];
+            const int stages = std::min((smem - kSplitFixed) / stage, kMaxStages);
+            const float block = std::max({share * T * 1.37e-3f, share * stage * 7.48e-6f, 1.42f / stages, 0.13f});
+            const float stream = std::max(static_cast<float>(g.N) * g.K * 0.139e-6f, rounds * ((KB + splits - 1) / splits) * block);
+            offer(2.3f + stream + rounds * (share * T * 12.5e-3f + 1.f) - 1.f + (splits > 1 ? 0.87f + 0.27f * (splits - 1) : 0.f) +
+                      (group == 2 ? 0.63f : 0.f),
+                  Plan{group, T, splits, smem});
+          }
+        }
+      if (rows <= 128) break;
+    }
+  return best;
+}
+
+template <int OUT, bool SILU, int CG>
+static void launch_split(const Args& g, const Plan& p, cudaStream_t st) {
+
+  constexpr int kElem = OUT == kF32 ? 4 : 2;
+  constexpr int kChan = (SILU ? 64 : 128) * CG;
+  SplitArgs a;
+  const int T = p.T;
+  a.g = g;
+  a.n_out = SILU ? g.N / 2 : g.N;
+  a.KB = (g.K + kBK - 1) / kBK;
+  a.T = T;
+  a.nb = T > 256 ? T / 2 : T;
+  a.tiles_m = (g.M - 1) / T + 1;
+  a.splits = p.splits;
+  a.stage_bytes = (128 + T / CG) * kBK;
+  a.stages = std::min({(p.smem - kSplitFixed) / a.stage_bytes, (a.KB + a.splits - 1) / a.splits, kMaxStages});
+  a.bar_off = std::max(a.stages * a.stage_bytes, T * 512);
+  a.tmem_cols = 32;
+  while (a.tmem_cols < T) a.tmem_cols *= 2;
+  a.wide = a.n_out % 4 == 0 && (reinterpret_cast<uintptr_t>(g.c) & (4 * kElem - 1)) == 0;
+  a.err = wait_error_flag();
+  const int smem = a.bar_off + kSplitFixed;
+  CUtensorMap amap, wmap;
+  if (!map_rows(&amap, g.a, g.M, g.K, a.nb / CG) || !map_rows(&wmap, g.w, g.N, g.K, SILU ? 64 : 128) || !a.err) {
+    set_error(2, "gemm_i8: cuTensorMapEncodeTiled failed");
+    return;
+  }
+  auto kern = split_kernel<OUT, SILU, CG>;
+  static OncePerDevice sized;
+  if (!allow_smem(sized, kern, kMaxSmem)) return;
+  const int tiles_n = (a.n_out - 1) / kChan + 1;
+  const cudaError_t e = launch_pdl_cluster(kern, dim3(tiles_n * a.tiles_m * a.splits * CG), dim3(kSplitThreads), smem, st,
+                                           dim3(a.splits * CG), wmap, amap, a);
+  if (e != cudaSuccess) set_error(2, cudaGetErrorString(e));
+  B200_CUDA_LAUNCH_CHECK();
+}
+
+template <int OUT, bool SILU>
+static void launch(const Args& g, cudaStream_t st) {
+  // Rows without tensor cores while the weights are few enough that a launch's start and end count (us, against the split kernel): one row
+  // of 6 144 x 4 096 6.5 and 8.2, 4 096 x 14 336 10.9 and 13.1, 28 672 x 4 096 23.0 and 22.0; two rows of 6 144 x 4 096 6.7 and 8.3, 4 096 x
+  // 14 336 13.8 and 13.2.
+  const int64_t weights = static_cast<int64_t>(g.N) * g.K;
+  if (g.M == 1 && weights <= 100 << 20) return launch_gemv<OUT, SILU, 1>(g, st);
+  if (g.M == 2 && weights <= 32 << 20) return launch_gemv<OUT, SILU, 2>(g, st);
+  const Plan p = plan(g);
+  if (p.group == 0) launch_pairs<OUT, SILU>(g, p.T, st);
+  else if (p.group == 1) launch_split<OUT, SILU, 1>(g, p, st);
+  else launch_split<OUT, SILU, 2>(g, p, st);
 }
 
 template <int OUT>
@@ -86,11 +832,8 @@ static void gemm(const Args& g, int epilogue, int64_t stream) {
                  "gemm_i8: rows and weights must be 16-byte aligned");
   B200_CHECK_ARG(epilogue == B200_EPI_NONE || (silu && g.N % 2 == 0), "gemm_i8: unknown epilogue, or an odd number of gate and up rows");
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const int n_out = silu ? g.N / 2 : g.N;
-  const dim3 grid((n_out + 63) / 64, (g.M + 63) / 64);
-  if (silu) launch_pdl(simple_kernel<OUT, true>, grid, dim3(256), 0, st, g);
-  else launch_pdl(simple_kernel<OUT, false>, grid, dim3(256), 0, st, g);
-  B200_CUDA_LAUNCH_CHECK();
+  if (silu) launch<OUT, true>(g, st);
+  else launch<OUT, false>(g, st);
 }
 
 }  // namespace gemm8
