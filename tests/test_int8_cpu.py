@@ -66,7 +66,7 @@ def ops(lib, monkeypatch):
         raise AssertionError("a call that should have been refused reached the library")
 
     monkeypatch.setattr(o, "_on_device", contiguous)
-    monkeypatch.setattr(o, "_stream", launched)
+    monkeypatch.setattr(o._lib, "check", launched)
     return o
 
 

@@ -116,7 +116,8 @@ def wna16_dequant(w_packed, scales, qzeros, *, k: int, n: int, bits=4, group_siz
 
 
 # ------------------------------------------------------------------ linear layers in 8-bit integers
-# Small calls cost what the host does: entry points are looked up once, every tensor is asked twice at most.
+# Small calls cost what the host does (a launch 2.4 us, a tensor 1.5): entry points are looked up once, tensors asked as little as
+# their checks need.
 _i8_entries = {}
 
 
@@ -133,47 +134,54 @@ def _i8_entry(stem: str, dtype):
     return fn
 
 
-def _on_device(*ts):
-    """Kernels go to the current device's stream: what they read and write lies there, without gaps."""
+def _on_device(*ts) -> int:
+    """Kernels go to the current device's stream, whose handle is returned: what they read and write lies there, without gaps."""
     dev = torch.cuda.current_device()
     for t in ts:
-        if t is not None and not (t.get_device() == dev and t.is_contiguous()):
+        if t.get_device() != dev or not t.is_contiguous():
             raise ValueError(f"b200 ops need contiguous CUDA tensors of the current device, cuda:{dev}; got one on {t.device} with "
                              f"strides {t.stride()}")
+    return _stream() if _raw_stream is None else _raw_stream(dev)
 
 
-def _expect(t, shape, dtype, what):
-    if t.dtype != dtype or t.shape != shape:
-        raise ValueError(f"{what} must be {shape} in {dtype}, got {tuple(t.shape)} in {t.dtype}")
+def _refuse(t, shape, dtype, what):
+    raise ValueError(f"{what} must be {tuple(shape)} in {dtype}, got {tuple(t.shape)} in {t.dtype}")
 
 
-def _i8_rows(x, out, scales, w=None, residual=None):
-    """Checks of what becomes int8 rows; rows, width, and the tensors of the codes and scales."""
-    if x.dim() != 2:
-        raise ValueError(f"rows must be [rows, width], got {tuple(x.shape)}")
-    shape = rows, width = x.shape
-    if w is not None:
-        _expect(w, (width,), x.dtype, "weight")
-    if residual is not None:
-        _expect(residual, shape, x.dtype, "residual")
-    if out is not None:
-        _expect(out, shape, torch.int8, "out")
-    if scales is not None:
-        _expect(scales, (rows,), torch.float32, "scales")
-    _on_device(x, w, residual, out, scales)
+def _i8_results(x, out, scales):
+    """The tensors of the codes and of the scales of rows x, checked where they are given."""
+    shape = x.shape
     if out is None:
         out = torch.empty_like(x, dtype=torch.int8)
+    else:
+        _on_device(out)
+        if out.shape != shape or out.dtype != torch.int8:
+            _refuse(out, shape, torch.int8, "out")
     if scales is None:
-        scales = torch.empty(rows, dtype=torch.float32, device=x.device)
-    return rows, width, out, scales
+        return out, torch.empty(shape[0], dtype=torch.float32, device=x.device)
+    _on_device(scales)
+    if scales.shape != shape[:1] or scales.dtype != torch.float32:
+        _refuse(scales, shape[:1], torch.float32, "scales")
+    return out, scales
+
+
+def _i8_norm_checks(x, w):
+    if x.dim() != 2:
+        raise ValueError(f"rows must be [rows, width], got {tuple(x.shape)}")
+    if w.shape != x.shape[1:] or w.dtype != x.dtype:
+        _refuse(w, x.shape[1:], x.dtype, "weight")
 
 
 def quant_rows_i8(x, out=None, scales=None):
     """Rows [R, W] (fp16 / bf16) to int8 codes and a scale per row (fp32): value = code * scale, codes = round(127 x / max|x|), ties
     to even, exactly.  Activations before an int8 product, and weights [N, K] when they are loaded.  Returns (codes, scales)."""
     fn = _i8_entry("b200_quant_rows_i8", x.dtype)
-    rows, width, out, scales = _i8_rows(x, out, scales)
-    fn(out.data_ptr(), scales.data_ptr(), x.data_ptr(), rows, width, _stream())
+    stream = _on_device(x)
+    if x.dim() != 2:
+        raise ValueError(f"rows must be [rows, width], got {tuple(x.shape)}")
+    out, scales = _i8_results(x, out, scales)
+    rows, width = x.shape
+    fn(out.data_ptr(), scales.data_ptr(), x.data_ptr(), rows, width, stream)
     _lib.check()
     return out, scales
 
@@ -181,8 +189,11 @@ def quant_rows_i8(x, out=None, scales=None):
 def rmsnorm_i8(x, w, eps, out=None, scales=None):
     """rmsnorm(x) * w as int8 codes and a scale per token, without a 16-bit rounding between.  Returns (codes, scales)."""
     fn = _i8_entry("b200_rmsnorm_i8", x.dtype)
-    rows, width, out, scales = _i8_rows(x, out, scales, w)
-    fn(out.data_ptr(), scales.data_ptr(), x.data_ptr(), w.data_ptr(), rows, width, eps, _stream())
+    stream = _on_device(x, w)
+    _i8_norm_checks(x, w)
+    out, scales = _i8_results(x, out, scales)
+    rows, width = x.shape
+    fn(out.data_ptr(), scales.data_ptr(), x.data_ptr(), w.data_ptr(), rows, width, eps, stream)
     _lib.check()
     return out, scales
 
@@ -190,8 +201,13 @@ def rmsnorm_i8(x, w, eps, out=None, scales=None):
 def add_rmsnorm_i8(residual, x, w, eps, out=None, scales=None):
     """residual += x (in place); rmsnorm(residual) * w as int8 codes and a scale per token.  Returns (codes, scales)."""
     fn = _i8_entry("b200_add_rmsnorm_i8", x.dtype)
-    rows, width, out, scales = _i8_rows(x, out, scales, w, residual)
-    fn(out.data_ptr(), scales.data_ptr(), residual.data_ptr(), x.data_ptr(), w.data_ptr(), rows, width, eps, _stream())
+    stream = _on_device(residual, x, w)
+    _i8_norm_checks(x, w)
+    if residual.shape != x.shape or residual.dtype != x.dtype:
+        _refuse(residual, x.shape, x.dtype, "residual")
+    out, scales = _i8_results(x, out, scales)
+    rows, width = x.shape
+    fn(out.data_ptr(), scales.data_ptr(), residual.data_ptr(), x.data_ptr(), w.data_ptr(), rows, width, eps, stream)
     _lib.check()
     return out, scales
 
@@ -201,26 +217,32 @@ def gemm_i8(x, x_scales, w_nk, w_scales, bias=None, epilogue=EPI_NONE, dtype=tor
     type: y = (x @ w^T) * x_scales * w_scales + bias, exact int32 sums, one rounding.  EPI_SILU_MUL: weights [gate | up],
     y [M, N / 2] = silu(gate) * up.  K is a multiple of 16.  `dtype`: of the output, float16, bfloat16 or float32."""
     fn = _i8_entry("b200_gemm_i8", dtype)
-    if x.dim() != 2 or w_nk.dim() != 2:
-        raise ValueError(f"rows [M, K] and weights [N, K] are needed, got {tuple(x.shape)} and {tuple(w_nk.shape)}")
-    (m, k), n = x.shape, w_nk.shape[0]
-    _expect(x, (m, k), torch.int8, "rows")
-    _expect(w_nk, (n, k), torch.int8, "weights")
-    _expect(x_scales, (m,), torch.float32, "rows' scales")
-    _expect(w_scales, (n,), torch.float32, "weights' scales")
+    stream = _on_device(x, x_scales, w_nk, w_scales)
+    if x.dim() != 2 or w_nk.dim() != 2 or x.dtype != torch.int8 or w_nk.dtype != torch.int8 or x.shape[1:] != w_nk.shape[1:]:
+        raise ValueError(f"int8 rows [M, K] and weights [N, K] are needed, got {tuple(x.shape)} in {x.dtype} and "
+                         f"{tuple(w_nk.shape)} in {w_nk.dtype}")
+    m, k = x.shape
+    n = w_nk.shape[0]
+    if x_scales.shape != (m,) or x_scales.dtype != torch.float32:
+        _refuse(x_scales, (m,), torch.float32, "rows' scales")
+    if w_scales.shape != (n,) or w_scales.dtype != torch.float32:
+        _refuse(w_scales, (n,), torch.float32, "weights' scales")
     if bias is not None:
-        _expect(bias, (n,), dtype, "bias")
+        _on_device(bias)
+        if bias.shape != (n,) or bias.dtype != dtype:
+            _refuse(bias, (n,), dtype, "bias")
     cols = n
     if epilogue != EPI_NONE:
         if epilogue != EPI_SILU_MUL or n % 2:
             raise ValueError(f"gemm_i8: epilogue {epilogue} with {n} weight rows")
         cols = n // 2
-    if out is not None:
-        _expect(out, (m, cols), dtype, "out")
-    _on_device(x, x_scales, w_nk, w_scales, bias, out)
     if out is None:
         out = torch.empty((m, cols), dtype=dtype, device=x.device)
-    fn(x.data_ptr(), x_scales.data_ptr(), w_nk.data_ptr(), w_scales.data_ptr(), _p(bias), out.data_ptr(), m, n, k, epilogue, _stream())
+    else:
+        _on_device(out)
+        if out.shape != (m, cols) or out.dtype != dtype:
+            _refuse(out, (m, cols), dtype, "out")
+    fn(x.data_ptr(), x_scales.data_ptr(), w_nk.data_ptr(), w_scales.data_ptr(), _p(bias), out.data_ptr(), m, n, k, epilogue, stream)
     _lib.check()
     return out
 
