@@ -161,7 +161,7 @@ def _case(m, n, k, dtype, bias, seed=0):
 def _check_product(y, a, sa, w, sw, bias, dtype, silu=False):
     acc = a.double() @ w.double().t()                    # exact: below 2^53
     p = acc * sa.double()[:, None] * sw.double()
-    b = torch.zeros(w.shape[0], dtype=torch.float64) if bias is None else bias.double()
+    b = torch.zeros(w.shape[0], dtype=torch.float64, device=w.device) if bias is None else bias.double()
     v = p + b
     off = 4 * U * (p.abs() + b.abs())                    # conversion of the sum, two scales, the bias
     if silu:
@@ -175,7 +175,7 @@ def _check_product(y, a, sa, w, sw, bias, dtype, silu=False):
         want = v
     half = torch.finfo(dtype).eps / 2
     tol = off + (0 if dtype == F32 else half * (want.abs() + off)) + torch.finfo(dtype).tiny * half
-    err = (y.double().cpu() - want).abs()
+    err = (y.double().to(want.device) - want).abs()
     assert y.dtype == dtype and y.shape == want.shape
     assert bool((err <= tol).all()), f"{int((err > tol).sum())} of {err.numel()} off, first {(err > tol).nonzero()[0].tolist()}"
 
@@ -208,6 +208,25 @@ def test_gated_products(ops, m, n, k, dtype):
     c = [t.cuda() for t in (a, sa, w, sw)]
     _check_product(ops.gemm_i8(*c, dtype=dtype, epilogue=ops.EPI_SILU_MUL), a, sa, w, sw, None, dtype, True)
     _check_product(ops.gemm_i8(*c, dtype=dtype, bias=bias.cuda(), epilogue=ops.EPI_SILU_MUL), a, sa, w, sw, bias, dtype, True)
+
+
+# shapes on every side of what decides how a product is cut: few and many tiles, short and long K, rows in one part and several
+CUTS = [(3, 130, 272), (3, 130, 2064), (3, 130, 4096), (3, 130, 8192), (3, 4096, 2064), (3, 8192, 8192), (40, 130, 272), (40, 130, 2064),
+        (40, 130, 4096), (40, 130, 8192), (40, 2048, 8192), (40, 5000, 2064), (70, 130, 2064), (100, 130, 272), (100, 130, 2064),
+        (100, 130, 4096), (100, 130, 8192), (100, 3000, 8192), (100, 5000, 4096), (100, 6144, 4096), (129, 3000, 4096),
+        (129, 3000, 8192), (200, 1000, 8192), (200, 3000, 4096), (257, 1536, 8192), (257, 10240, 272), (257, 10240, 1024),
+        (300, 1536, 4096), (300, 10240, 272), (300, 10240, 1024), (333, 2048, 8192), (500, 5000, 1024), (500, 10240, 272),
+        (600, 10240, 272), (700, 5000, 272), (700, 8192, 272), (900, 130, 272), (900, 130, 4096), (900, 130, 8192),
+        (900, 1000, 4096), (900, 1536, 272), (900, 1536, 1024), (900, 1536, 4096), (900, 5000, 272), (900, 5000, 1024)]
+
+
+@pytest.mark.parametrize("m,n,k", CUTS)
+def test_products_however_cut(ops, m, n, k):
+    a, sa, w, sw, bias = (t.cuda() for t in _case(m, n, k, BF16, True))
+    _check_product(ops.gemm_i8(a, sa, w, sw, bias=bias, dtype=BF16), a, sa, w, sw, bias, BF16)
+    _check_product(ops.gemm_i8(a, sa, w, sw, dtype=F32), a, sa, w, sw, None, F32)
+    sw = sw * 4
+    _check_product(ops.gemm_i8(a, sa, w, sw, bias=bias, dtype=BF16, epilogue=ops.EPI_SILU_MUL), a, sa, w, sw, bias, BF16, True)
 
 
 @pytest.mark.parametrize("m", [1, 32, 130, 300])

@@ -337,26 +337,33 @@ pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CU
 }
 
 // ------------------------------------------------------------------ few rows
-// A tile is 128 CG weight rows (lanes of the accumulator; gated: of every block's 128, 64 are gate rows and 64 the up rows of the
-// same channels) by T rows of a (its columns, in one product or two of nb).  CG = 2: pairs of blocks, each with its own weight rows
-// and half of the rows of a in shared memory.  `splits` parts of a cluster share K evenly; their int32 sums, exact in any order, meet
-// in shared memory: every block writes its own there, then takes its share of the rows of a from all that have the same weight
-// rows, scales and stores.  No workspace, one launch.
+// A tile is 128 CG weight rows (lanes of the accumulator) by T rows of a (its columns, in one product or two of nb).  CG = 2: pairs of
+// blocks, each with its own weight rows and half of the rows of a in shared memory.  Gated: every 32 lanes are 16 gate rows and the
+// up rows of the same channels, which a shuffle brings together.  `splits` parts of a cluster share K evenly and the tile's rows
+// of a in turn (`share` each): the others' int32 sums, exact in any order, come to a part's shared memory, its own stay in tensor
+// memory.  No workspace, one launch.
 constexpr int kMaxSmem = 227 * 1024, kSplitThreads = 320, kMaxStages = 24, kMaxT = 384;
 constexpr int kSplitFixed = 1024 + 512 + kMaxT * 4;          // alignment; barriers; the tile's a_scales
 
 struct SplitArgs {
   Args g;
-  int n_out, KB, T, nb, tiles_m, splits, stages, stage_bytes, bar_off, tmem_cols, wide;
+  int n_out, KB, T, nb, tiles_m, splits, share, stages, stage_bytes, sums_off, bar_off, tmem_cols;
   int* err;
 };
 
-template <int V> struct Int { static constexpr int value = V; };
-
-__device__ __forceinline__ uint4 ld_cluster_v4(uint32_t addr) {
-  uint4 r;
-  asm volatile("ld.shared::cluster.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(addr) : "memory");
-  return r;
+__device__ __forceinline__ void tmem_ld_x8(uint32_t taddr, uint32_t (&v)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_cg2(void* dst, const CUtensorMap* m, uint32_t bar_cluster_addr, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar_cluster_addr), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
 }
 
 template <int OUT, bool SILU, int CG>
@@ -375,7 +382,7 @@ split_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
   const int rank = C > 1 ? static_cast<int>(cluster_ctarank()) : 0, part = rank / CG, half = rank % CG, tile = blockIdx.x / C;
   const int tn = tile / a.tiles_m, tm = tile - tn * a.tiles_m;
   constexpr int kChan = SILU ? 64 : 128;           // output channels of a block
-  const int n0 = (tn * CG + half) * kChan, m0 = tm * a.T;
+  const int n0 = (tn * CG + half) * kChan, m0 = tm * a.T, rows = min(a.T, a.g.M - m0);
   const int kb0 = part * a.KB / S, kb1 = (part + 1) * a.KB / S;
 
   pdl_trigger();
@@ -398,7 +405,7 @@ split_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
   }
   tc_fence_before();
   __syncthreads();
-  if constexpr (CG == 2) {                         // the other block's barriers are there
+  if (C > 1) {                                     // the other blocks run, and a pair's barriers are there
     cluster_arrive();
     cluster_wait();
   }
@@ -406,21 +413,6 @@ split_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
   pdl_wait();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_ptr, 0);
 
-  // a lane's four channels at the end; gated: half a warp per row of a, the same lane has gate and up
-  const int ch = SILU ? (lane & 15) * 4 : lane * 4, n = n0 + ch;
-  float sw[4], su[4], bw[4] = {}, bu[4] = {};
-  auto channel_scales = [&] {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const bool in = n + j < a.n_out;
-      sw[j] = in ? a.g.w_scales[n + j] : 0.f;
-      if (SILU) su[j] = in ? a.g.w_scales[a.n_out + n + j] : 0.f;
-      if (a.g.bias && in) {
-        bw[j] = load_elem<OUT>(a.g.bias, n + j);
-        if (SILU) bu[j] = load_elem<OUT>(a.g.bias, a.n_out + n + j);
-      }
-    }
-  };
   if (warp == 0) {
     // ------------------------------------------------------------ operands
     int s = 0, armed = 0;
@@ -434,14 +426,22 @@ split_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
         if constexpr (CG == 2) {                   // both blocks' bytes count on the first one's barrier
           if (half == 0) mbar_arrive_expect_tx(&full[s], bytes);
           const uint32_t bar = mapa_shared(smem_u32(&full[s]), rank & ~1);
-          tma_load_2d_cg2(dst, &wmap, bar, kb * kBK, n0);
-          if (SILU) tma_load_2d_cg2(dst + 64 * kBK, &wmap, bar, kb * kBK, a.n_out + n0);
+          if constexpr (SILU) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) tma_load_3d_cg2(dst + i * 32 * kBK, &wmap, bar, kb * kBK, n0 + i * 16, 0);
+          } else {
+            tma_load_2d_cg2(dst, &wmap, bar, kb * kBK, n0);
+          }
           for (int i = 0; i < a.T; i += a.nb, tok += a.nb / 2 * kBK)
             tma_load_2d_cg2(tok, &amap, bar, kb * kBK, m0 + i + half * (a.nb / 2));
         } else {
           mbar_arrive_expect_tx(&full[s], bytes);
-          tma_load_2d(dst, &wmap, &full[s], kb * kBK, n0);
-          if (SILU) tma_load_2d(dst + 64 * kBK, &wmap, &full[s], kb * kBK, a.n_out + n0);
+          if constexpr (SILU) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) tma_load_3d(dst + i * 32 * kBK, &wmap, &full[s], kb * kBK, n0 + i * 16, 0);
+          } else {
+            tma_load_2d(dst, &wmap, &full[s], kb * kBK, n0);
+          }
           for (int i = 0; i < a.T; i += a.nb, tok += a.nb * kBK) tma_load_2d(tok, &amap, &full[s], kb * kBK, m0 + i);
         }
       }
@@ -475,105 +475,104 @@ split_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
       if (*fail) mbar_wait_limited(done, 0, nullptr, a.err);    // products in flight end before TMEM is given back
       __syncwarp();
     }
-  } else {
-    // this block's sums, [row of a][weight row], where the stages were: all of them have been read.  Two warps per quarter of the lanes.
-    for (int r = threadIdx.x - 64; r < a.T; r += kSplitThreads - 64) row_scale[r] = m0 + r < a.g.M ? a.g.a_scales[m0 + r] : 0.f;
-    channel_scales();
+  }
+  // ------------------------------------------------------------ sums meet
+  // A thread's weight row, as the accumulator's lanes have it; two warps per 32 lanes take eight columns in turn.
+  const int q4 = warp & 3, chan = SILU ? q4 * 16 + (lane & 15) : q4 * 32 + lane, n = n0 + chan;
+  const int first = warp < 6 ? 0 : 8, mine = part * a.share, mine_end = min(mine + a.share, rows);
+  const uint32_t acc = tmem + (static_cast<uint32_t>(q4 * 32) << 16);
+  const uint32_t lane_off = static_cast<uint32_t>(q4 * 32 + lane) * 4;
+  float sw = 0.f, bw = 0.f;
+  if (warp > 1) {
+    const int at = n + (SILU && lane >= 16 ? a.n_out : 0);
+    if (n < a.n_out) {
+      sw = a.g.w_scales[at];
+      if (a.g.bias) bw = load_elem<OUT>(a.g.bias, at);
+    }
+    for (int r = threadIdx.x - 64; r < a.T; r += kSplitThreads - 64) row_scale[r] = r < rows ? a.g.a_scales[m0 + r] : 0.f;
     mbar_wait_limited(done, 0, fail, a.err);
     __syncwarp();
     tc_fence_after();
-    const int q4 = warp & 3;
-    uint32_t* sums = reinterpret_cast<uint32_t*>(smem) + q4 * 32 + lane;
-    for (int c = warp < 6 ? 0 : 32; c < a.T; c += 64) {
-      uint32_t v[32];
-      tmem_ld_x32(tmem + (static_cast<uint32_t>(q4 * 32) << 16) + c, v);
-      tc_wait_ld();
-#pragma unroll
-      for (int j = 0; j < 32; ++j) sums[(c + j) * 128] = v[j];
-    }
   }
-  if (warp < 2) channel_scales();
-  tc_fence_before();
-  if (C > 1) {
+  if (S == 1) {
+    __syncthreads();
+  } else {
+    if (a.sums_off == 0) {                         // the sums take the stages' place: every block's products have ended
+      __syncwarp();
+      cluster_arrive();
+      cluster_wait();
+    }
+    if (warp > 1) {
+      const uint32_t sums = smem_u32(smem) + a.sums_off + lane_off;
+      for (int c = first; c < rows; c += 16) {
+        const int owner = c / a.share;
+        if (owner == part) continue;
+        uint32_t v[8];
+        tmem_ld_x8(acc + c, v);
+        const uint32_t dst = mapa_shared(sums, owner * CG + half) +
+                             static_cast<uint32_t>((part < owner ? part : part - 1) * a.share + c - owner * a.share) * 512;
+        tc_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) st_cluster_u32(dst + j * 512, v[j]);
+      }
+    }
     __syncwarp();
     cluster_arrive();
     cluster_wait();
-  } else {
-    __syncthreads();
   }
-  constexpr int kPer = SILU ? 2 : 1, kStep = kSplitThreads / 32 * kPer;      // rows of a per warp at a time; of a turn
-  const int r0 = part * a.T / S, r1 = min((part + 1) * a.T / S, a.g.M - m0);
-  const uint32_t here = smem_u32(smem);
-  // kBatch turns at once, sums of kParts blocks at once
-  auto finish = [&](auto batch, auto parts) {
-    constexpr int kBatch = decltype(batch)::value, kParts = decltype(parts)::value;
-#pragma unroll 1
-    for (int rb = r0 + warp * kPer + (SILU ? lane >> 4 : 0); rb < r1; rb += kBatch * kStep) {
-      int x[kBatch][4] = {};
-      [[maybe_unused]] int y[SILU ? kBatch : 1][4] = {};
-      for (int p0 = 0; p0 < S; p0 += kParts) {       // asked for at once: another block's memory answers in 0.4 us
-        uint4 v[kParts][kBatch];
-        [[maybe_unused]] uint4 w[kParts][SILU ? kBatch : 1];
+  // ------------------------------------------------------------ scales and stores
+  if (warp > 1) {
+    constexpr int kElem = OUT == kF32 ? 4 : 2;
+    const uint32_t* sums = reinterpret_cast<const uint32_t*>(smem + a.sums_off + lane_off);
+    // gated: lanes 0-15 have gates and take the first of two rows, lanes 16-31 ups and the second
+    uint8_t* out = static_cast<uint8_t*>(a.g.c) + (static_cast<size_t>(m0 + mine + first + (SILU ? lane >> 4 : 0)) * a.n_out + n) * kElem;
+    const size_t pitch = static_cast<size_t>(a.n_out) * kElem * (SILU ? 2 : 1);
+    const int live = n < a.n_out ? mine_end - (SILU ? lane >> 4 : 0) : 0;      // rows from here on are not this thread's
+    uint32_t next[8];
+    if (mine + first < mine_end) tmem_ld_x8(acc + mine + first, next);
+    for (int c = mine + first; c < mine_end; c += 16, out += static_cast<size_t>(a.n_out) * kElem * 16) {
+      const float4 s0 = *reinterpret_cast<const float4*>(row_scale + c), s1 = *reinterpret_cast<const float4*>(row_scale + c + 4);
+      const float sa[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+      uint32_t v[8];
+      tc_wait_ld();
 #pragma unroll
-        for (int q = 0; q < kParts; ++q) {
-          const uint32_t base = (C > 1 ? mapa_shared(here, min(p0 + q, S - 1) * CG + half) : here) + ch * 4;
+      for (int j = 0; j < 8; ++j) v[j] = next[j];
+      if (c + 16 < mine_end) tmem_ld_x8(acc + c + 16, next);       // under this turn's arithmetic
+      for (int p = 0; p < S - 1; ++p)
 #pragma unroll
-          for (int i = 0; i < kBatch; ++i) {
-            const bool there = p0 + q < S && rb + i * kStep < r1;
-            v[q][i] = there ? ld_cluster_v4(base + (rb + i * kStep) * 512) : make_uint4(0, 0, 0, 0);
-            if constexpr (SILU) w[q][i] = there ? ld_cluster_v4(base + (rb + i * kStep) * 512 + 64 * 4) : make_uint4(0, 0, 0, 0);
-          }
-        }
+        for (int j = 0; j < 8; ++j) v[j] += sums[(p * a.share + c - mine + j) * 128];
+      float f[8];
 #pragma unroll
-        for (int q = 0; q < kParts; ++q)
+      for (int j = 0; j < 8; ++j) f[j] = scaled(static_cast<int>(v[j]), sa[j], sw);
+      if (a.g.bias) {
 #pragma unroll
-          for (int i = 0; i < kBatch; ++i) {
-            x[i][0] += static_cast<int>(v[q][i].x); x[i][1] += static_cast<int>(v[q][i].y);
-            x[i][2] += static_cast<int>(v[q][i].z); x[i][3] += static_cast<int>(v[q][i].w);
-            if constexpr (SILU) {
-              y[i][0] += static_cast<int>(w[q][i].x); y[i][1] += static_cast<int>(w[q][i].y);
-              y[i][2] += static_cast<int>(w[q][i].z); y[i][3] += static_cast<int>(w[q][i].w);
-            }
-          }
+        for (int j = 0; j < 8; ++j) f[j] = __fadd_rn(f[j], bw);
       }
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const int r = rb + i * kStep;
-        if (r >= r1) break;
-        const float sa = row_scale[r];
-        float f[4];
+      uint8_t* dst = out;
+      if constexpr (SILU) {
+        float y[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          f[j] = scaled(x[i][j], sa, sw[j]);
-          if (a.g.bias) f[j] = __fadd_rn(f[j], bw[j]);
-          if constexpr (SILU) {
-            float u = scaled(y[i][j], sa, su[j]);
-            if (a.g.bias) u = __fadd_rn(u, bu[j]);
-            f[j] = silu_mul(f[j], u);
-          }
+          const float other = __shfl_xor_sync(0xffffffffu, lane < 16 ? f[2 * j + 1] : f[2 * j], 16);
+          y[j] = silu_mul(lane < 16 ? f[2 * j] : other, lane < 16 ? other : f[2 * j + 1]);
         }
-        const size_t at = static_cast<size_t>(m0 + r) * a.n_out + n;
-        if (a.wide) {                                // four channels are all there or none
-          if (n < a.n_out) {
-            if constexpr (OUT == kF32) *reinterpret_cast<float4*>(static_cast<float*>(a.g.c) + at) = make_float4(f[0], f[1], f[2], f[3]);
-            else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.g.c) + at) =
-                make_uint2(pack16x2<OUT == kBF16>(f[0], f[1]), pack16x2<OUT == kBF16>(f[2], f[3]));
-          }
-        } else {
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (n + j < a.n_out) store_elem<OUT>(a.g.c, at + j, f[j]);
-        }
+        for (int j = 0; j < 4; ++j, dst += pitch)
+          if (c + 2 * j < live) store_elem<OUT>(dst, 0, y[j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j, dst += pitch)
+          if (c + j < live) store_elem<OUT>(dst, 0, f[j]);
       }
     }
-  };
-  if (S == 1) finish(Int<SILU ? 1 : 4>{}, Int<1>{});
-  else if (S == 2) finish(Int<SILU ? 2 : 8>{}, Int<2>{});
-  else finish(Int<SILU ? 1 : 4>{}, Int<4>{});
-  if (C > 1) {                                     // no block goes while another can read its sums; what it read is in use, the results
-    __syncwarp();                                  // that it stored need not have arrived (a release would wait for them: 0.7 us)
+  }
+  tc_fence_before();
+  if constexpr (CG == 2) {                         // neither of a pair goes while the other has its tensor memory
+    __syncthreads();
     asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     cluster_wait();
+  } else {
+    __syncthreads();
   }
   if (warp == 1) {
     tc_fence_after();
@@ -648,6 +647,14 @@ static bool map_rows(CUtensorMap* m, const void* base, int rows, int K, int box_
   return encode_tensor_map(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, es,
                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B) == CUDA_SUCCESS;
 }
+// gate and up rows as two planes: a box is 16 channels of both
+static bool map_gated(CUtensorMap* m, const void* base, int n_out, int K) {
+  const uint64_t dims[3] = {static_cast<uint64_t>(K), static_cast<uint64_t>(n_out), 2};
+  const uint64_t strides[2] = {static_cast<uint64_t>(K), static_cast<uint64_t>(n_out) * K};
+  const uint32_t box[3] = {kBK, 16, 2}, es[3] = {1, 1, 1};
+  return encode_tensor_map(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, es,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B) == CUDA_SUCCESS;
+}
 template <typename K>
 static bool allow_smem(OncePerDevice& once, K kern, int bytes) {
   int dev = 0;
@@ -716,6 +723,10 @@ struct Room {
   }
 };
 
+// Rows of a that a part of K finishes, and the bytes of the other parts' sums of them.
+constexpr int share_of(int T, int splits) { return ((T + splits - 1) / splits + 7) / 8 * 8; }
+constexpr int sums_bytes(int T, int splits) { return (splits - 1) * share_of(T, splits) * 512; }
+
 // What a product is cut into: `group` 0 pairs of blocks with tiles of 256 x T weight rows, 1 and 2 the split kernel with so many blocks
 // per tile and T rows of a.
 struct Plan {
@@ -723,14 +734,14 @@ struct Plan {
 };
 
 // The estimates (us) are fits to 311 shapes (8 to 4 096 rows, N and K from 256 to 28 672), each measured in every form; the form taken
-// costs 1.5 % more than the best one in the mean, 20 % at most.  A block of K takes as long as the tensor core, the L2 (7.5 ns a
-// KB) or the memory's answer over the stages that wait for it; weights come at 7.2 TB/s at best; an epilogue 12 ns a row; a meeting
-// of parts 0.9 us and 0.27 for each further part.  What the choice is worth, us: 257 rows of 4 096 x 14 336 pairs 42, one part 28,
-// two parts 19.3, four of half an SM 24; 1 003 of 10 240 x 8 192 pairs 62.6 (256 wide 64.3), split 72.5.
+// costs 1 % more than the best one in the mean, a sixth at most.  A block of K takes as long as the tensor core, the L2 (7.8 ns
+// a KB) or the memory's answer over the stages that wait for it; weights come at 7.4 TB/s at best; an epilogue 12 ns a row; a
+// meeting of parts 0.6 us where their sums have a place of their own, else 1.7, and 0.36 for each further part.  What the choice is
+// worth, us: 257 rows of 4 096 x 14 336 pairs 42, one part 28, two parts 18.7 - 20.1, four of half an SM 24; 1 003 of 10 240 x
+// 8 192 pairs 62.6 (256 wide 64.3), split 72.5.
 static Plan plan(const Args& g) {
   static const Room room;
   const int KB = (g.K + kBK - 1) / kBK;
-  const auto up = [](int x, int q) { return (x + q - 1) / q * q; };
   Plan best{0, 256, 1, 0};
   float least = 3.4e38f;
   const auto offer = [&](float us, const Plan& p) {
@@ -741,29 +752,29 @@ static Plan plan(const Args& g) {
   };
   if (g.M > 128)
     for (int bn = 64; bn <= 256; bn += 64) {
-      const int64_t tiles = (static_cast<int64_t>(g.M) + 255) / 256 * ((g.N + bn - 1) / bn), pairs = sm_count() / 2;
-      const float block = std::max(bn * 0.58e-3f, (128 + bn / 2) * kBK * 9.04e-6f);
-      offer(2.75f + static_cast<float>((tiles + pairs - 1) / pairs) * (KB * block + 1.f) + bn * 5.96e-3f, Plan{0, bn, 1, 0});
+      const int64_t tiles = (static_cast<int64_t>(g.M) + 255) / 256 * ((g.N - 1) / bn + 1), pairs = sm_count() / 2;
+      const float block = (128 + bn / 2) * kBK * 9.15e-6f;
+      offer(2.19f + static_cast<float>((tiles + pairs - 1) / pairs) * (KB * block + 1.11f) + bn * 9.4e-3f, Plan{0, bn, 1, 0});
     }
   if (g.M <= 1536)
     for (int parts = 1; parts <= 5; ++parts) {
       const int rows = (g.M + parts - 1) / parts;
       if (rows <= kMaxT)
         for (int group = 1; group <= 2; ++group) {
-          const int T = up(rows, rows > 256 || group == 2 ? 64 : 32);
-          const int64_t tiles = static_cast<int64_t>((g.N - 1) / (128 * group) + 1) * ((g.M + T - 1) / T);
+          const int unit = rows > 256 ? 64 : 32, T = (rows + unit - 1) / unit * unit;       // (a product's nb is a multiple of 32)
+          const int64_t tiles = static_cast<int64_t>((g.N - 1) / (128 * group) + 1) * ((g.M - 1) / T + 1);
           const int stage = (128 + T / group) * kBK;
           for (int splits = 1; splits * group <= 8 && splits <= KB; ++splits) {
             const int c = splits * group - 1;
             const bool whole = tiles <= room.whole[c];
-            if (!whole && T * 512 > kHalfSm - kSplitFixed) continue;
+            if (!whole && (T > 256 || sums_bytes(T, splits) > kHalfSm - kSplitFixed)) continue;      // (two blocks share tensor memory, too)
             const int share = whole ? 1 : 2, smem = whole ? kWholeSm : kHalfSm;
             const int64_t rounds = whole ? 1 : (tiles + room.half[c] - 1) / room.half[c];
             const int stages = std::min((smem - kSplitFixed) / stage, kMaxStages);
-            const float block = std::max({share * T * 1.37e-3f, share * stage * 7.48e-6f, 1.42f / stages, 0.13f});
-            const float stream = std::max(static_cast<float>(g.N) * g.K * 0.139e-6f, rounds * ((KB + splits - 1) / splits) * block);
-            offer(2.3f + stream + rounds * (share * T * 12.5e-3f + 1.f) - 1.f + (splits > 1 ? 0.87f + 0.27f * (splits - 1) : 0.f) +
-                      (group == 2 ? 0.63f : 0.f),
+            const float block = std::max({share * T * 1.21e-3f, share * stage * 7.63e-6f, 1.44f / stages});
+            const float stream = std::max(static_cast<float>(g.N) * g.K * 0.136e-6f, rounds * ((KB + splits - 1) / splits) * block);
+            offer(1.59f + stream + rounds * (share * T * 12.2e-3f + 0.88f) - 0.88f +
+                      (splits > 1 ? (T > 64 ? 1.65f : 0.53f) + 0.36f * (splits - 1) : 0.f) + (group == 2 ? 0.64f : 0.f),
                   Plan{group, T, splits, smem});
           }
         }
@@ -774,28 +785,29 @@ static Plan plan(const Args& g) {
 
 template <int OUT, bool SILU, int CG>
 static void launch_split(const Args& g, const Plan& p, cudaStream_t st) {
-
-  constexpr int kElem = OUT == kF32 ? 4 : 2;
   constexpr int kChan = (SILU ? 64 : 128) * CG;
   SplitArgs a;
-  const int T = p.T;
   a.g = g;
   a.n_out = SILU ? g.N / 2 : g.N;
   a.KB = (g.K + kBK - 1) / kBK;
-  a.T = T;
-  a.nb = T > 256 ? T / 2 : T;
-  a.tiles_m = (g.M - 1) / T + 1;
+  a.T = p.T;
+  a.nb = p.T > 256 ? p.T / 2 : p.T;
+  a.tiles_m = (g.M - 1) / p.T + 1;
   a.splits = p.splits;
-  a.stage_bytes = (128 + T / CG) * kBK;
-  a.stages = std::min({(p.smem - kSplitFixed) / a.stage_bytes, (a.KB + a.splits - 1) / a.splits, kMaxStages});
-  a.bar_off = std::max(a.stages * a.stage_bytes, T * 512);
+  a.share = share_of(p.T, p.splits);
+  a.stage_bytes = (128 + p.T / CG) * kBK;
+  // the other parts' sums have a place of their own where it is small, which saves a meeting of the blocks; else that of the stages
+  const int sums = sums_bytes(p.T, p.splits), own = p.splits > 1 && p.T <= 64 ? sums : 0;
+  a.stages = std::min({(p.smem - kSplitFixed - own) / a.stage_bytes, (a.KB + a.splits - 1) / a.splits, kMaxStages});
+  a.sums_off = own ? a.stages * a.stage_bytes : 0;
+  a.bar_off = own ? a.sums_off + own : std::max(a.stages * a.stage_bytes, sums);
   a.tmem_cols = 32;
-  while (a.tmem_cols < T) a.tmem_cols *= 2;
-  a.wide = a.n_out % 4 == 0 && (reinterpret_cast<uintptr_t>(g.c) & (4 * kElem - 1)) == 0;
+  while (a.tmem_cols < p.T) a.tmem_cols *= 2;
   a.err = wait_error_flag();
   const int smem = a.bar_off + kSplitFixed;
   CUtensorMap amap, wmap;
-  if (!map_rows(&amap, g.a, g.M, g.K, a.nb / CG) || !map_rows(&wmap, g.w, g.N, g.K, SILU ? 64 : 128) || !a.err) {
+  if (!map_rows(&amap, g.a, g.M, g.K, a.nb / CG) || !(SILU ? map_gated(&wmap, g.w, a.n_out, g.K) : map_rows(&wmap, g.w, g.N, g.K, 128)) ||
+      !a.err) {
     set_error(2, "gemm_i8: cuTensorMapEncodeTiled failed");
     return;
   }
