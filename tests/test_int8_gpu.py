@@ -339,9 +339,11 @@ def test_feed_forward_of_a_layer(ops, tokens, dtype):
         assert all(torch.equal(p, e) for p, e in zip(again, (*eager, r1)))
 
 
-def test_two_streams_at_once(ops):
-    """Calls on two streams share nothing: results are those of one after the other."""
-    cases = [_case(m, 2048, 1024, BF16, False, seed) for m, seed in ((32, 1), (300, 2))]
+@pytest.mark.parametrize("shapes", [((32, 2048, 1024), (300, 2048, 1024)), ((64, 4096, 128), (333, 1536, 256)), ((900, 1536, 128), (129, 3000, 4096))])
+def test_two_streams_at_once(ops, shapes):
+    """Calls on two streams share nothing: results are those of one after the other.  Clusters that want much tensor memory and little
+    shared memory, among them."""
+    cases = [_case(m, n, k, BF16, False, seed) for seed, (m, n, k) in enumerate(shapes)]
     cases = [[t.cuda() for t in c[:4]] for c in cases]
     want = [ops.gemm_i8(*c, dtype=BF16) for c in cases]
     streams = [torch.cuda.Stream() for _ in cases]
@@ -353,3 +355,49 @@ def test_two_streams_at_once(ops):
                 got[i].append(ops.gemm_i8(*c, dtype=BF16))
     torch.cuda.synchronize()
     assert all(torch.equal(y, w) for ys, w in zip(got, want) for y in ys)
+
+
+def test_first_call_within_a_capture(lib):
+    """A process whose first call is captured: what is set up once is no part of the graph."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = """
+import torch
+from vllm_rs_b200 import ops
+q = torch.randint(-127, 128, (300, 256), dtype=torch.int8, device="cuda"); w = torch.randint(-127, 128, (512, 256), dtype=torch.int8, device="cuda")
+s, t = torch.rand(300, device="cuda"), torch.rand(512, device="cuda")
+x = torch.randn(300, 256, device="cuda").half()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = [ops.gemm_i8(q[:m], s[:m], w, t, dtype=torch.float32) for m in (1, 2, 40, 300)]
+    c = ops.quant_rows_i8(x)
+graph.replay()
+z = [ops.gemm_i8(q[:m], s[:m], w, t, dtype=torch.float32) for m in (1, 2, 40, 300)]
+d = ops.quant_rows_i8(x)
+assert all(torch.equal(a, b) for a, b in zip((*y, *c), (*z, *d)))
+print("equal")
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "equal" in r.stdout, r.stderr[-2000:]
+
+
+def test_offsets_past_32_bits(ops):
+    """Rows whose elements lie past 2^31 and past 2^32 bytes, in codes, results and weights."""
+    rows, width = 140_000, 16_384
+    x = torch.zeros(rows, width, dtype=BF16, device="cuda")
+    last = _rows(3, 5, width, BF16)
+    x[-5:] = last.cuda()
+    q, s = ops.quant_rows_i8(x)
+    _check_rows((q[-5:], s[-5:]), last.float())
+    assert not q[:64].any() and not s[:-5].any()
+    del x, q, s
+    for m, n in ((80_000, 32_768), (1, 40_000_000), (30, 40_000_000), (300, 8_000_000)):
+        k = 128 if m == 1 else 64 if m == 30 else 16
+        a, sa, w, sw, _ = (None if t is None else t.cuda() for t in _case(min(m, 300), min(n, 32_768), k, F16, False))
+        a, sa = a.repeat(m // a.shape[0] + 1, 1)[:m].contiguous(), sa.repeat(m // sa.shape[0] + 1)[:m].contiguous()
+        w, sw = w.repeat(n // w.shape[0] + 1, 1)[:n].contiguous(), sw.repeat(n // sw.shape[0] + 1)[:n].contiguous()
+        y = ops.gemm_i8(a, sa, w, sw)
+        _check_product(y[-min(m, 70):, -1000:], a[-min(m, 70):], sa[-min(m, 70):], w[-1000:], sw[-1000:], None, F16)
+        _check_product(y[:min(m, 70), :1000], a[:min(m, 70)], sa[:min(m, 70)], w[:1000], sw[:1000], None, F16)
+        del y, w

@@ -133,7 +133,6 @@ pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CU
   const int rank = static_cast<int>(cluster_ctarank()), unit = blockIdx.x >> 1, units = gridDim.x >> 1;
   const int ntiles = a.tiles_m * a.tiles_n, cols = SILU ? a.bn / 2 : a.bn;
 
-  pdl_trigger();
   if (threadIdx.x == 0) {
     for (int s = 0; s < kPairStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
     for (int s = 0; s < 2; ++s) { mbar_init(&tfull[s], 1); mbar_init(&tempty[s], kEpiWarps * 2); }
@@ -152,6 +151,7 @@ pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CU
   cluster_arrive();                                // the other block's barriers are there
   cluster_wait();
   tc_fence_after();
+  pdl_trigger();                                   // (not before tensor memory is there: see smem_floor)
   pdl_wait();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_ptr, 0);
   // group_m row tiles, then the next weight tile: their rows stay in L2 while the weights pass once per group
@@ -385,7 +385,6 @@ split_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
   const int n0 = (tn * CG + half) * kChan, m0 = tm * a.T, rows = min(a.T, a.g.M - m0);
   const int kb0 = part * a.KB / S, kb1 = (part + 1) * a.KB / S;
 
-  pdl_trigger();
   if (threadIdx.x == 0) {
     for (int s = 0; s < a.stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
     mbar_init(done, 1);
@@ -410,6 +409,7 @@ split_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
     cluster_wait();
   }
   tc_fence_after();
+  pdl_trigger();                                   // (not before tensor memory is there: see smem_floor)
   pdl_wait();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_ptr, 0);
 
@@ -704,6 +704,13 @@ static void launch_gemv(const Args& g, cudaStream_t st) {
   B200_CUDA_LAUNCH_CHECK();
 }
 
+// Shared memory that a block asks for at least, so that the blocks on an SM never want more tensor memory together than there is: a
+// block that waits for columns while its cluster waits for it must not have them kept from it by a block that waits the same way
+// elsewhere.  Shared memory runs out as columns do (228 KB and 512), and what is left beside the kernels that take all columns
+// (195 KB and more) is too little for any block.  For the same reason the next kernel may only start once all columns are given out.
+constexpr int smem_floor(int tmem_cols) { return std::max(32 * 1024, 228 * 1024 / 512 * tmem_cols - 1024); }
+static_assert(smem_floor(512) <= kMaxSmem && smem_floor(256) <= 113 * 1024, "what can be asked for");
+
 // Blocks of the split kernel that an SM holds take all of its shared memory or half of it.
 constexpr int kWholeSm = 226 * 1024, kHalfSm = 113 * 1024;
 
@@ -804,7 +811,7 @@ static void launch_split(const Args& g, const Plan& p, cudaStream_t st) {
   a.tmem_cols = 32;
   while (a.tmem_cols < p.T) a.tmem_cols *= 2;
   a.err = wait_error_flag();
-  const int smem = a.bar_off + kSplitFixed;
+  const int smem = std::max(a.bar_off + kSplitFixed, smem_floor(a.tmem_cols));
   CUtensorMap amap, wmap;
   if (!map_rows(&amap, g.a, g.M, g.K, a.nb / CG) || !(SILU ? map_gated(&wmap, g.w, a.n_out, g.K) : map_rows(&wmap, g.w, g.N, g.K, 128)) ||
       !a.err) {
