@@ -118,20 +118,22 @@ def wna16_dequant(w_packed, scales, qzeros, *, k: int, n: int, bits=4, group_siz
 # ------------------------------------------------------------------ linear layers in 8-bit integers
 # Small calls cost what the host does (a launch 2.4 us, a tensor 1.5): entry points are looked up once, tensors asked as little as
 # their checks need.
-_i8_entries = {}
+class _Entries(dict):
+    """The flavours of an entry point by dtype, found when they are first asked for."""
+
+    def __init__(self, stem: str, also=()):
+        super().__init__()
+        self.stem, self.names = stem, {torch.float16: "_f16", torch.bfloat16: "_bf16", **dict(also)}
+
+    def __missing__(self, dtype):
+        if dtype not in self.names:
+            raise TypeError(f"{self.stem}: {dtype} is none of {', '.join(map(str, self.names))}")
+        self[dtype] = fn = getattr(_lib.lib(), self.stem + self.names[dtype])
+        return fn
 
 
-def _i8_entry(stem: str, dtype):
-    """The flavour of an entry point that `dtype` (16 bits; results of products also float32) names."""
-    fn = _i8_entries.get((stem, dtype))
-    if fn is None:
-        names = {torch.float16: "_f16", torch.bfloat16: "_bf16"}
-        if stem == "b200_gemm_i8":
-            names[torch.float32] = "_f32"
-        if dtype not in names:
-            raise TypeError(f"{stem}: {dtype} is none of {', '.join(map(str, names))}")
-        fn = _i8_entries[stem, dtype] = getattr(_lib.lib(), stem + names[dtype])
-    return fn
+_QUANT_ROWS_I8, _RMSNORM_I8, _ADD_RMSNORM_I8 = (_Entries(f"b200_{n}_i8") for n in ("quant_rows", "rmsnorm", "add_rmsnorm"))
+_GEMM_I8 = _Entries("b200_gemm_i8", also={torch.float32: "_f32"})
 
 
 def _on_device(*ts) -> int:
@@ -153,6 +155,8 @@ def _i8_results(x, out, scales):
     shape = x.shape
     if out is None:
         out = torch.empty_like(x, dtype=torch.int8)
+        if scales is None:
+            return out, torch.empty(shape[0], dtype=torch.float32, device=x.device)
     else:
         _on_device(out)
         if out.shape != shape or out.dtype != torch.int8:
@@ -175,7 +179,7 @@ def _i8_norm_checks(x, w):
 def quant_rows_i8(x, out=None, scales=None):
     """Rows [R, W] (fp16 / bf16) to int8 codes and a scale per row (fp32): value = code * scale, codes = round(127 x / max|x|), ties
     to even, exactly.  Activations before an int8 product, and weights [N, K] when they are loaded.  Returns (codes, scales)."""
-    fn = _i8_entry("b200_quant_rows_i8", x.dtype)
+    fn = _QUANT_ROWS_I8[x.dtype]
     stream = _on_device(x)
     if x.dim() != 2:
         raise ValueError(f"rows must be [rows, width], got {tuple(x.shape)}")
@@ -188,7 +192,7 @@ def quant_rows_i8(x, out=None, scales=None):
 
 def rmsnorm_i8(x, w, eps, out=None, scales=None):
     """rmsnorm(x) * w as int8 codes and a scale per token, without a 16-bit rounding between.  Returns (codes, scales)."""
-    fn = _i8_entry("b200_rmsnorm_i8", x.dtype)
+    fn = _RMSNORM_I8[x.dtype]
     stream = _on_device(x, w)
     _i8_norm_checks(x, w)
     out, scales = _i8_results(x, out, scales)
@@ -200,7 +204,7 @@ def rmsnorm_i8(x, w, eps, out=None, scales=None):
 
 def add_rmsnorm_i8(residual, x, w, eps, out=None, scales=None):
     """residual += x (in place); rmsnorm(residual) * w as int8 codes and a scale per token.  Returns (codes, scales)."""
-    fn = _i8_entry("b200_add_rmsnorm_i8", x.dtype)
+    fn = _ADD_RMSNORM_I8[x.dtype]
     stream = _on_device(residual, x, w)
     _i8_norm_checks(x, w)
     if residual.shape != x.shape or residual.dtype != x.dtype:
@@ -216,7 +220,7 @@ def gemm_i8(x, x_scales, w_nk, w_scales, bias=None, epilogue=EPI_NONE, dtype=tor
     """int8 rows [M, K] times int8 weights [N, K], scales fp32 per row and per output channel, optional bias [N] in the output's
     type: y = (x @ w^T) * x_scales * w_scales + bias, exact int32 sums, one rounding.  EPI_SILU_MUL: weights [gate | up],
     y [M, N / 2] = silu(gate) * up.  K is a multiple of 16.  `dtype`: of the output, float16, bfloat16 or float32."""
-    fn = _i8_entry("b200_gemm_i8", dtype)
+    fn = _GEMM_I8[dtype]
     stream = _on_device(x, x_scales, w_nk, w_scales)
     if x.dim() != 2 or w_nk.dim() != 2 or x.dtype != torch.int8 or w_nk.dtype != torch.int8 or x.shape[1:] != w_nk.shape[1:]:
         raise ValueError(f"int8 rows [M, K] and weights [N, K] are needed, got {tuple(x.shape)} in {x.dtype} and "
