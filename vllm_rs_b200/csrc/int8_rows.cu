@@ -16,6 +16,7 @@
 // A row of zeros has scale 0 and codes 0.  A row with a NaN or an infinity has scale NaN and codes 0: all that is computed from
 // it is NaN.
 #include "../../include/b200_vllm.h"
+#include <algorithm>
 #include "common.cuh"
 #include "f32x2.cuh"
 
@@ -155,47 +156,29 @@ __device__ __forceinline__ void store8_any(int8_t* p, const uint2& q) {
   }
 }
 
-// Thread `tid` of `n` that share a row: piece c of it, eight neighbours.  VEC: the width is a multiple of 8 and all begins on 16 bytes
-// (codes: on eight); else the row's last piece goes element by element.
-template <bool VEC>
-struct Piece {
-  int at, width;
-  __device__ __forceinline__ Piece(int tid, int c, int n, int width_) : at((c * n + tid) * 8), width(width_) {}
-  __device__ __forceinline__ uint4 load(const uint16_t* p) const {
-    if constexpr (VEC) {
-      return at < width ? *reinterpret_cast<const uint4*>(p + at) : make_uint4(0, 0, 0, 0);
-    } else {
-      if (at + 8 <= width) return load8_any(p + at);
-      uint32_t h[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) h[j] = at + j < width ? p[at + j] : 0u;
-      return make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
-    }
-  }
-  __device__ __forceinline__ void store(uint16_t* p, const uint4& v) const {
-    if constexpr (VEC) {
-      if (at < width) *reinterpret_cast<uint4*>(p + at) = v;
-    } else if (at + 8 <= width) {
-      store8_any(p + at, v);
-    } else {
-      const uint32_t h[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (at + j < width) p[at + j] = static_cast<uint16_t>(h[j >> 1] >> (16 * (j & 1)));
-    }
-  }
-  __device__ __forceinline__ void store(int8_t* p, const uint2& q) const {
-    if constexpr (VEC) {
-      if (at < width) *reinterpret_cast<uint2*>(p + at) = q;
-    } else if (at + 8 <= width) {
-      store8_any(p + at, q);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (at + j < width) p[at + j] = static_cast<int8_t>((j < 4 ? q.x : q.y) >> (8 * (j & 3)));
-    }
-  }
-};
+// How rows lie.  kEven: the width is a multiple of 8, all begins on 16 bytes (codes: on eight).  kFrame: the tensors begin so and rows
+// anywhere; pieces of eight are cut where memory has its 16 bytes, which is the same place in rows, residual and codes, up to seven
+// elements before and after them go one by one, and only the weight lies off.  kAny: the rest.
+enum Lay { kEven, kFrame, kAny };
+
+// The weight's eight elements at an even address: five words about them, asked for at once and shifted in place later.
+struct Words { uint32_t w[5]; };
+__device__ __forceinline__ Words ask_words(const uint16_t* p) {
+  const bool odd = reinterpret_cast<uintptr_t>(p) & 2;
+  const uint32_t* q = reinterpret_cast<const uint32_t*>(p - (odd ? 1 : 0));
+  Words r;
+  r.w[0] = odd ? p[0] : q[0];
+  r.w[1] = q[1];
+  r.w[2] = q[2];
+  r.w[3] = q[3];
+  r.w[4] = odd ? p[7] : 0u;
+  return r;
+}
+__device__ __forceinline__ uint4 in_place(const Words& r, const uint16_t* p) {
+  const uint32_t s = (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 2) * 8;
+  return make_uint4(__funnelshift_r(r.w[0] << s, r.w[1], s), __funnelshift_r(r.w[1], r.w[2], s), __funnelshift_r(r.w[2], r.w[3], s),
+                    __funnelshift_r(r.w[3], r.w[4], s));
+}
 
 // max(|a|, |b|, |c|), NaN where one is
 __device__ __forceinline__ float max3_abs(float a, float b, float c) {
@@ -231,7 +214,7 @@ __device__ __forceinline__ uint4 add8(uint4 a, const uint4& r) {
 }
 
 // A block per row, or (WARP) a warp, NC pieces of eight elements per thread (0: as many as it takes, read twice).
-template <bool BF, bool NORM, bool ADD, bool VEC, bool WARP, int NC>
+template <bool BF, bool NORM, bool ADD, Lay LAY, bool WARP, int NC>
 __global__ void __launch_bounds__(WARP ? 32 * kWarpRows : NC ? 512 : 1024) rows_i8_kernel(const Args a) {
   pdl_trigger();
   pdl_wait();
@@ -244,37 +227,75 @@ __global__ void __launch_bounds__(WARP ? 32 * kWarpRows : NC ? 512 : 1024) rows_
   const uint16_t* x = a.x + at;
   uint16_t* res = ADD ? a.residual + at : nullptr;
   int8_t* out = a.out + at;
+  // whole pieces are [head, body); an edge's element belongs to one of the first sixteen threads
+  const int head = LAY == kFrame ? min(static_cast<int>(-at & 7), a.width) : 0;
+  const int body = LAY == kEven ? a.width : head + (a.width - head) / 8 * 8;
+  const int edge = LAY == kEven ? a.width : tid < 8 ? (tid < head ? tid : a.width) : tid < 16 ? body + tid - 8 : a.width;
+  const bool has_edge = edge < a.width;
   f2 squares = pack2(0.f, 0.f);
-  float most = 0.f;
+  float most = 0.f, edge_t = 0.f;
 
   f2 t[NC ? NC : 1][4];
   const uint4 none = make_uint4(0, 0, 0, 0);
+  auto fetch = [&](const uint16_t* p, int i) {
+    if constexpr (LAY == kAny) return load8_any(p + i);
+    else return *reinterpret_cast<const uint4*>(p + i);
+  };
+  auto ask_weight = [&](int i) {
+    if constexpr (LAY == kEven) {
+      const uint4 v = *reinterpret_cast<const uint4*>(a.w + i);
+      return Words{{v.x, v.y, v.z, v.w, 0u}};
+    } else {
+      return ask_words(a.w + i);
+    }
+  };
+  auto weight = [&](const Words& r, int i) {
+    if constexpr (LAY == kEven) return make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]);
+    else return in_place(r, a.w + i);
+  };
+  auto keep = [&](int i, const uint4& v) {                   // the residual
+    if constexpr (LAY == kAny) store8_any(res + i, v);
+    else *reinterpret_cast<uint4*>(res + i) = v;
+  };
+  if (has_edge) {
+    uint32_t v = x[edge];
+    if constexpr (ADD) {
+      v = add16x2<BF>(v, res[edge]);
+      res[edge] = static_cast<uint16_t>(v);
+    }
+    f2 e[4];
+    take8<BF, NORM>(make_uint4(v & 0xffffu, 0, 0, 0), make_uint4(NORM ? a.w[edge] : 0u, 0, 0, 0), e, squares, most);
+    float rest;
+    unpack2(e[0], edge_t, rest);
+  }
   if constexpr (NC) {
-    uint4 v[NC], r[ADD ? NC : 1], w[NORM ? NC : 1];
+    uint4 v[NC], r[ADD ? NC : 1];
+    Words w[NORM ? NC : 1];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const Piece<VEC> pc(tid, c, n, a.width);
-      v[c] = pc.load(x);
-      if constexpr (ADD) r[c] = pc.load(res);
-      if constexpr (NORM) w[c] = pc.load(a.w);
+      const int i = head + (c * n + tid) * 8;
+      const bool in = i < body;
+      v[c] = in ? fetch(x, i) : none;
+      if constexpr (ADD) r[c] = in ? fetch(res, i) : none;
+      if constexpr (NORM) w[c] = in ? ask_weight(i) : Words{};
     }
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
+      const int i = head + (c * n + tid) * 8;
       if constexpr (ADD) {
         v[c] = add8<BF>(v[c], r[c]);
-        Piece<VEC>(tid, c, n, a.width).store(res, v[c]);
+        if (i < body) keep(i, v[c]);
       }
-      take8<BF, NORM>(v[c], NORM ? w[NORM ? c : 0] : none, t[c], squares, most);
+      take8<BF, NORM>(v[c], NORM ? weight(w[NORM ? c : 0], i) : none, t[c], squares, most);
     }
   } else {
-    for (int c = 0; c * n * 8 < a.width; ++c) {
-      const Piece<VEC> pc(tid, c, n, a.width);
-      uint4 v = pc.load(x);
+    for (int i = head + tid * 8; i < body; i += n * 8) {
+      uint4 v = fetch(x, i);
       if constexpr (ADD) {
-        v = add8<BF>(v, pc.load(res));
-        pc.store(res, v);
+        v = add8<BF>(v, fetch(res, i));
+        keep(i, v);
       }
-      take8<BF, NORM>(v, NORM ? pc.load(a.w) : none, t[0], squares, most);
+      take8<BF, NORM>(v, NORM ? weight(ask_weight(i), i) : none, t[0], squares, most);
     }
   }
   float ss = 0.f;
@@ -302,15 +323,27 @@ __global__ void __launch_bounds__(WARP ? 32 * kWarpRows : NC ? 512 : 1024) rows_
     a.scales[row] = finite ? s / 127.f : __uint_as_float(0x7fc00000u);
   }
   const Coder<BF || !NORM> code(finite ? A : 0.f);
+  auto put = [&](int i, const f2 (&v)[4]) {
+    const uint2 q = finite ? code(v) : make_uint2(0, 0);
+    if constexpr (LAY == kAny) store8_any(out + i, q);
+    else *reinterpret_cast<uint2*>(out + i) = q;
+  };
   if constexpr (NC) {
 #pragma unroll
-    for (int c = 0; c < NC; ++c) Piece<VEC>(tid, c, n, a.width).store(out, finite ? code(t[c]) : make_uint2(0, 0));
-  } else {
-    for (int c = 0; c * n * 8 < a.width; ++c) {
-      const Piece<VEC> pc(tid, c, n, a.width);
-      take8<BF, NORM>(pc.load(ADD ? res : x), NORM ? pc.load(a.w) : none, t[0], squares, most);
-      pc.store(out, finite ? code(t[0]) : make_uint2(0, 0));
+    for (int c = 0; c < NC; ++c) {
+      const int i = head + (c * n + tid) * 8;
+      if (i < body) put(i, t[c]);
     }
+  } else {
+    for (int i = head + tid * 8; i < body; i += n * 8) {
+      take8<BF, NORM>(fetch(ADD ? res : x, i), NORM ? weight(ask_weight(i), i) : none, t[0], squares, most);
+      put(i, t[0]);
+    }
+  }
+  if (has_edge) {
+    const f2 zero = pack2(0.f, 0.f);
+    const f2 e[4] = {pack2(edge_t, 0.f), zero, zero, zero};
+    out[edge] = finite ? static_cast<int8_t>(code(e).x) : int8_t{0};
   }
 }
 
@@ -319,32 +352,32 @@ __global__ void __launch_bounds__(WARP ? 32 * kWarpRows : NC ? 512 : 1024) rows_
 //                    residual up to 512 wide: 13.7 and 17.9, but 1 024 wide 20.6 and 18.3.  Below 1 000 rows there is nothing in it.
 //   pieces a thread  many rows: to codes, 8 192 x 14 336 with 8 / 4 pieces 57 / 66, x 4 096 with 4 / 2 30.5 / 32.7; with the residual,
 //                    whose loads are twice as many, 8 192 x 8 192 with 2 / 4 69.3 / 70.9.  Few rows: as many threads as there are.
-// Rows that do not lie on 16 bytes take more instructions than the loads hide: 2 pieces, or the loop (8 192 x 16 383: 141).
-template <bool BF, bool NORM, bool ADD, bool VEC>
+// Rows that begin off 16 bytes: 8 192 x 16 383 to codes 76 (141 by the accesses that every row's own alignment allows), x 8 191 with the
+// residual 95.
+template <bool BF, bool NORM, bool ADD, Lay LAY>
 static void launch(const Args& a, cudaStream_t st) {
-  const int pieces = (a.width - 1) / 8 + 1;
+  const int pieces = (a.width - 1) / 8 + 1;        // (whole ones are no more)
   const auto go = [&](auto kern, int blocks, int threads) {
     launch_pdl(kern, dim3(blocks), dim3(threads), 0, st, a);
     B200_CUDA_LAUNCH_CHECK();
   };
+  if constexpr (LAY == kAny) return go(rows_i8_kernel<BF, NORM, ADD, LAY, false, 0>, a.rows, std::min((pieces + 31) / 32 * 32, 1024));
   if (a.rows >= 1000 && pieces <= (ADD ? 64 : 128)) {
     const int blocks = (a.rows - 1) / kWarpRows + 1;
-    if (pieces <= 32) go(rows_i8_kernel<BF, NORM, ADD, VEC, true, 1>, blocks, 32 * kWarpRows);
-    else go(rows_i8_kernel<BF, NORM, ADD, VEC, true, 4>, blocks, 32 * kWarpRows);
+    if (pieces <= 32) go(rows_i8_kernel<BF, NORM, ADD, LAY, true, 1>, blocks, 32 * kWarpRows);
+    else go(rows_i8_kernel<BF, NORM, ADD, LAY, true, 4>, blocks, 32 * kWarpRows);
     return;
   }
   const bool many = a.rows > 2 * sm_count();
-  const int most = !many || ADD || !VEC ? 512 : NORM ? 256 : 128;      // threads
+  const int most = !many || ADD ? 512 : NORM ? 256 : 128;      // threads
   int nc = many && ADD ? 2 : 1;
   while (nc < 8 && pieces > nc * most) nc *= 2;
   const auto threads = [&] { return ((pieces - 1) / nc / 32 + 1) * 32; };
-  if (pieces > 512 * nc || (!VEC && nc > 2)) return go(rows_i8_kernel<BF, NORM, ADD, VEC, false, 0>, a.rows, 1024);
-  if (nc == 1) return go(rows_i8_kernel<BF, NORM, ADD, VEC, false, 1>, a.rows, threads());
-  if (nc == 2) return go(rows_i8_kernel<BF, NORM, ADD, VEC, false, 2>, a.rows, threads());
-  if constexpr (VEC) {
-    if (nc == 4) return go(rows_i8_kernel<BF, NORM, ADD, VEC, false, 4>, a.rows, threads());
-    go(rows_i8_kernel<BF, NORM, ADD, VEC, false, 8>, a.rows, threads());
-  }
+  if (pieces > 512 * nc) return go(rows_i8_kernel<BF, NORM, ADD, LAY, false, 0>, a.rows, 1024);
+  if (nc == 1) return go(rows_i8_kernel<BF, NORM, ADD, LAY, false, 1>, a.rows, threads());
+  if (nc == 2) return go(rows_i8_kernel<BF, NORM, ADD, LAY, false, 2>, a.rows, threads());
+  if (nc == 4) return go(rows_i8_kernel<BF, NORM, ADD, LAY, false, 4>, a.rows, threads());
+  go(rows_i8_kernel<BF, NORM, ADD, LAY, false, 8>, a.rows, threads());
 }
 
 template <bool BF, bool NORM, bool ADD>
@@ -352,11 +385,12 @@ static void rows_i8(void* out, float* scales, void* residual, const void* x, con
                     int64_t stream) {
   const Args a{static_cast<int8_t*>(out), scales, static_cast<uint16_t*>(residual), static_cast<const uint16_t*>(x),
                static_cast<const uint16_t*>(w), rows, width, eps};
-  const uintptr_t wide = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(residual) | reinterpret_cast<uintptr_t>(w);
-  const bool vec = width % 8 == 0 && (wide & 15) == 0 && (reinterpret_cast<uintptr_t>(out) & 7) == 0;
+  const auto on16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+  const bool frame = on16(x) && on16(residual) && (reinterpret_cast<uintptr_t>(out) & 7) == 0;
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (vec) launch<BF, NORM, ADD, true>(a, st);
-  else launch<BF, NORM, ADD, false>(a, st);
+  if (!frame) launch<BF, NORM, ADD, kAny>(a, st);
+  else if (width % 8 || !on16(w)) launch<BF, NORM, ADD, kFrame>(a, st);
+  else launch<BF, NORM, ADD, kEven>(a, st);
 }
 
 }  // namespace rows8
