@@ -241,6 +241,17 @@ def test_largest_sums(ops, m):
         assert bool((y.double().cpu() == float(torch.tensor(-128.0 * v * k, dtype=F32))).all())
 
 
+@pytest.mark.parametrize("silu", [False, True], ids=["plain", "gated"])
+@pytest.mark.parametrize("n,k", [(640, 4112), (2048, 272), (6144, 1024)])
+def test_results_do_not_depend_on_the_batch(ops, n, k, silu):
+    """A row's results are the same bits alone and in any batch: sums are exact, and what follows is the same operations."""
+    a, sa, w, sw, bias = (t.cuda() for t in _case(1700, n, k, BF16, True))
+    run = lambda r: ops.gemm_i8(a[r], sa[r], w, sw, bias=bias, dtype=BF16, epilogue=int(silu))          # noqa: E731
+    whole = run(slice(0, 1700))
+    for m in (1, 2, 3, 31, 64, 100, 129, 200, 257, 384, 600, 1100):
+        assert torch.equal(run(slice(7, 7 + m)), whole[7:7 + m]), m
+
+
 def test_scales_that_are_not_finite(ops):
     a, sa, w, sw, _ = _case(40, 200, 256, F16, False)
     sa[3], sa[5], sw[7] = torch.nan, 0.0, torch.nan

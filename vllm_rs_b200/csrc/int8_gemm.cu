@@ -6,10 +6,10 @@
 // `plan` choose, with what was measured there):
 //   gemv_kernel    one row or two: dp4a, weights straight to registers.  Bound: HBM, and the launch's start and end.
 //   split_kernel   up to some thousand rows: one tile per block or pair of blocks, K shared by the blocks of a cluster.  Bound: HBM up to
-//                  some 100 rows (32 x 28 672 x 4 096 gated 21.6 us, floor 18.2; x 128 256 85.9 and 82.9), then what the L2
-//                  delivers to the SMs (257 x 4 096 x 14 336: 21.6 us, HBM alone 9.9).
+//                  some 100 rows (32 x 28 672 x 4 096 gated 22.0 us, floor 18.2; x 128 256 86 and 82.9), then what the L2
+//                  delivers to the SMs (257 x 4 096 x 14 336: 21.9 us, HBM alone 9.9).
 //   pair_kernel    many rows: persistent pairs of blocks.  Bound: the tensor cores, in long runs under the power cap (8 192 x 28 672 x
-//                  4 096 gated: 2.9 - 3.1 PFLOP/s; cuBLAS in bf16 reaches 1.64 in a burst, 1.37 sustained).
+//                  4 096 gated: 2.8 - 3.3 PFLOP/s; cuBLAS in bf16 reaches 1.64 in a burst, 1.37 sustained).
 #include "../../include/b200_vllm.h"
 #include <algorithm>
 #include "common.cuh"
@@ -355,8 +355,8 @@ __device__ __forceinline__ void tmem_ld_x8(uint32_t taddr, uint32_t (&v)[8]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(taddr) : "memory");
 }
-__device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) {
-  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+__device__ __forceinline__ void st_cluster_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared::cluster.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 __device__ __forceinline__ void tma_load_3d_cg2(void* dst, const CUtensorMap* m, uint32_t bar_cluster_addr, int c0, int c1, int c2) {
   asm volatile(
@@ -501,7 +501,9 @@ split_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
   const int q4 = warp & 3, chan = SILU ? q4 * 16 + (lane & 15) : q4 * 32 + lane, n = n0 + chan;
   const int first = warp < 6 ? 0 : 8, mine = part * a.share, mine_end = min(mine + a.share, rows);
   const uint32_t acc = tmem + (static_cast<uint32_t>(q4 * 32) << 16);
-  const uint32_t lane_off = static_cast<uint32_t>(q4 * 32 + lane) * 4;
+  // sums on their way: eight columns of 128 lanes are 4 KB, a thread's eight two pieces of 16 bytes (the thread that takes them has the
+  // same lane and columns)
+  const uint32_t lane_off = static_cast<uint32_t>(q4 * 1024 + lane * 16);
   float sw = 0.f, bw = 0.f;
   if (warp > 1) {
     const int at = n + (SILU && lane >= 16 ? a.n_out : 0);
@@ -532,8 +534,8 @@ split_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
         const uint32_t dst = mapa_shared(sums, owner * CG + half) +
                              static_cast<uint32_t>((part < owner ? part : part - 1) * a.share + c - owner * a.share) * 512;
         tc_wait_ld();
-#pragma unroll
-        for (int j = 0; j < 8; ++j) st_cluster_u32(dst + j * 512, v[j]);
+        st_cluster_v4(dst, v[0], v[1], v[2], v[3]);
+        st_cluster_v4(dst + 512, v[4], v[5], v[6], v[7]);
       }
     }
     __syncwarp();
@@ -543,7 +545,7 @@ split_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
   // ------------------------------------------------------------ scales and stores
   if (warp > 1) {
     constexpr int kElem = OUT == kF32 ? 4 : 2;
-    const uint32_t* sums = reinterpret_cast<const uint32_t*>(smem + a.sums_off + lane_off);
+    const uint8_t* sums = smem + a.sums_off + lane_off;
     // gated: lanes 0-15 have gates and take the first of two rows, lanes 16-31 ups and the second
     uint8_t* out = static_cast<uint8_t*>(a.g.c) + (static_cast<size_t>(m0 + mine + first + (SILU ? lane >> 4 : 0)) * a.n_out + n) * kElem;
     const size_t pitch = static_cast<size_t>(a.n_out) * kElem * (SILU ? 2 : 1);
@@ -558,9 +560,12 @@ split_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = next[j];
       if (c + 16 < mine_end) tmem_ld_x8(acc + c + 16, next);       // under this turn's arithmetic
-      for (int p = 0; p < S - 1; ++p)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] += sums[(p * a.share + c - mine + j) * 128];
+      for (int p = 0; p < S - 1; ++p) {
+        const uint4* q = reinterpret_cast<const uint4*>(sums + (p * a.share + c - mine) * 512);
+        const uint4 lo = q[0], hi = q[32];
+        v[0] += lo.x; v[1] += lo.y; v[2] += lo.z; v[3] += lo.w;
+        v[4] += hi.x; v[5] += hi.y; v[6] += hi.z; v[7] += hi.w;
+      }
       float f[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) f[j] = scaled(static_cast<int>(v[j]), sa[j], sw);
