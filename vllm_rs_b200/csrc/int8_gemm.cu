@@ -4,7 +4,7 @@
 //
 // Three forms, all with the same arithmetic behind the exact sums, so that a result does not depend on which one ran (`launch` and
 // `plan` choose, with what was measured there):
-//   gemv_kernel    one row or two: dp4a, weights straight to registers.  Bound: HBM, and the launch's start and end.
+//   gemv_kernel    up to four rows: dp4a, weights straight to registers.  Bound: HBM, and the launch's start and end.
 //   split_kernel   up to some thousand rows: one tile per block or pair of blocks, K shared by the blocks of a cluster.  Bound: HBM up to
 //                  some 100 rows (32 x 28 672 x 4 096 gated 22.0 us, floor 18.2; x 128 256 86 and 82.9), then what the L2
 //                  delivers to the SMs (257 x 4 096 x 14 336: 21.9 us, HBM alone 9.9).
@@ -606,13 +606,18 @@ split_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
   }
 }
 
-// ------------------------------------------------------------------ one row to a few
-// A block has eight weight rows (gated: four gate rows and the up rows of the same channels); its warps take 512 of K in turn, eight
-// 16-byte loads a lane at once, four products per dp4a.
-constexpr int kGemvThreads = 256, kGemvRows = 8;
+// ------------------------------------------------------------------ one row to four
+// A block has `Rows` weight rows (gated: half of them gate rows, half the up rows of the same channels); its warps take 512 of K in turn,
+// `Rows` 16-byte loads a lane at once, four products per dp4a.  Blocks are small and many per SM, so that enough loads are under way
+// and the last ones end together (one row of 4 096 x 14 336, us: 256 threads with 4 rows, 8 blocks per SM 10.5; with 8 rows, 4 blocks
+// 10.9; 128 threads with 8 rows 12.5.  Two rows: 128 threads with 8 rows 10.4, 256 with 8 13.3, with 4 13.0).
+template <int MT> struct Gemv {
+  static constexpr int kThreads = MT == 1 ? 256 : 128, kRows = MT == 1 ? 4 : 8, kPerSm = MT == 1 ? 8 : MT == 2 ? 5 : 4;
+};
 
 template <int OUT, bool SILU, int MT>
-__global__ void __launch_bounds__(kGemvThreads, MT == 1 ? 4 : 3) gemv_kernel(const Args g, int n_out) {
+__global__ void __launch_bounds__(Gemv<MT>::kThreads, Gemv<MT>::kPerSm) gemv_kernel(const Args g, int n_out) {
+  constexpr int kGemvThreads = Gemv<MT>::kThreads, kGemvRows = Gemv<MT>::kRows;
   constexpr int kChan = SILU ? kGemvRows / 2 : kGemvRows;
   __shared__ int red[kGemvThreads / 32][kGemvRows * MT];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n0 = blockIdx.x * kChan;
@@ -727,9 +732,9 @@ static void launch_pairs(const Args& g, int bn, cudaStream_t st) {
 
 template <int OUT, bool SILU, int MT>
 static void launch_gemv(const Args& g, cudaStream_t st) {
-  constexpr int kChan = SILU ? kGemvRows / 2 : kGemvRows;
+  constexpr int kChan = SILU ? Gemv<MT>::kRows / 2 : Gemv<MT>::kRows;
   const int n_out = SILU ? g.N / 2 : g.N;
-  launch_pdl(gemv_kernel<OUT, SILU, MT>, dim3((n_out - 1) / kChan + 1), dim3(kGemvThreads), 0, st, g, n_out);
+  launch_pdl(gemv_kernel<OUT, SILU, MT>, dim3((n_out - 1) / kChan + 1), dim3(Gemv<MT>::kThreads), 0, st, g, n_out);
   B200_CUDA_LAUNCH_CHECK();
 }
 
@@ -860,12 +865,11 @@ static void launch_split(const Args& g, const Plan& p, cudaStream_t st) {
 
 template <int OUT, bool SILU>
 static void launch(const Args& g, cudaStream_t st) {
-  // Rows without tensor cores while the weights are few enough that a launch's start and end count (us, against the split kernel): one row
-  // of 6 144 x 4 096 6.5 and 8.2, 4 096 x 14 336 10.9 and 13.1, 28 672 x 4 096 23.0 and 22.0; two rows of 6 144 x 4 096 6.7 and 8.3, 4 096 x
-  // 14 336 13.8 and 13.2.
-  const int64_t weights = static_cast<int64_t>(g.N) * g.K;
-  if (g.M == 1 && weights <= 100 << 20) return launch_gemv<OUT, SILU, 1>(g, st);
-  if (g.M == 2 && weights <= 32 << 20) return launch_gemv<OUT, SILU, 2>(g, st);
+  // Up to four rows go without tensor cores (us, against the split kernel): one row of 6 144 x 4 096 5.7 and 8.0, 28 672 x 4 096 gated
+  // 20.5 and 21.9; two rows 6.8 and 8.3, 20.2 and 21.5; four rows 7.2 and 8.3, but 23.0 and 21.5.
+  if (g.M == 1) return launch_gemv<OUT, SILU, 1>(g, st);
+  if (g.M == 2) return launch_gemv<OUT, SILU, 2>(g, st);
+  if (g.M <= 4 && static_cast<int64_t>(g.N) * g.K <= 100 << 20) return launch_gemv<OUT, SILU, 4>(g, st);
   const Plan p = plan(g);
   if (p.group == 0) launch_pairs<OUT, SILU>(g, p.T, st);
   else if (p.group == 1) launch_split<OUT, SILU, 1>(g, p, st);
