@@ -2,9 +2,10 @@
 //   y[m, n] = (sum_k a[m, k] w[n, k]) * a_scales[m] * w_scales[n] (+ bias[n])      int32 sums, exact up to K = 131056
 // rounded once to fp16, bf16 or fp32.  SiLU: w holds gate rows, then as many up rows; out[m, n] = silu(gate) * up of the fp32 values.
 //
-// Three forms, all with the same arithmetic behind the exact sums, so that a result does not depend on which one ran (`launch` and
+// Four forms, all with the same arithmetic behind the exact sums, so that a result does not depend on which one ran (`launch` and
 // `plan` choose, with what was measured there):
-//   gemv_kernel    up to four rows: dp4a, weights straight to registers.  Bound: HBM, and the launch's start and end.
+//   gemv_kernel    one row or two: dp4a, weights straight to registers.  Bound: HBM, and the launch's start and end.
+//   few_kernel     up to sixteen rows: mma.sync, weights straight to its fragments.  Bound as above.
 //   split_kernel   up to some thousand rows: one tile per block or pair of blocks, K shared by the blocks of a cluster.  Bound: HBM up to
 //                  some 100 rows (32 x 28 672 x 4 096 gated 22.0 us, floor 18.2; x 128 256 86 and 82.9), then what the L2
 //                  delivers to the SMs (257 x 4 096 x 14 336: 21.9 us, HBM alone 9.9).
@@ -606,13 +607,13 @@ split_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
   }
 }
 
-// ------------------------------------------------------------------ one row to four
+// ------------------------------------------------------------------ one row or two
 // A block has `Rows` weight rows (gated: half of them gate rows, half the up rows of the same channels); its warps take 512 of K in turn,
 // `Rows` 16-byte loads a lane at once, four products per dp4a.  Blocks are small and many per SM, so that enough loads are under way
 // and the last ones end together (one row of 4 096 x 14 336, us: 256 threads with 4 rows, 8 blocks per SM 10.5; with 8 rows, 4 blocks
 // 10.9; 128 threads with 8 rows 12.5.  Two rows: 128 threads with 8 rows 10.4, 256 with 8 13.3, with 4 13.0).
 template <int MT> struct Gemv {
-  static constexpr int kThreads = MT == 1 ? 256 : 128, kRows = MT == 1 ? 4 : 8, kPerSm = MT == 1 ? 8 : MT == 2 ? 5 : 4;
+  static constexpr int kThreads = MT == 1 ? 256 : 128, kRows = MT == 1 ? 4 : 8, kPerSm = MT == 1 ? 8 : 5;
 };
 
 template <int OUT, bool SILU, int MT>
@@ -667,6 +668,82 @@ __global__ void __launch_bounds__(Gemv<MT>::kThreads, Gemv<MT>::kPerSm) gemv_ker
       int s = 0;
 #pragma unroll
       for (int i = 0; i < kGemvThreads / 32; ++i) s += red[i][m * kGemvRows + h * kChan + t % kChan];
+      v[h] = scaled(s, g.a_scales[m], g.w_scales[h * n_out + n]);
+      if (g.bias) v[h] = __fadd_rn(v[h], load_elem<OUT>(g.bias, h * n_out + n));
+    }
+    store_elem<OUT>(g.c, static_cast<size_t>(m) * n_out + n, SILU ? silu_mul(v[0], v[1]) : v[0]);
+  }
+}
+
+// ------------------------------------------------------------------ up to sixteen rows
+// A block has 16 weight rows (gated: 8 gate rows and the up rows of the same channels), its warps take 128 of K in turn, and a product is
+// one warp's: weights go from memory to the fragments of mma.sync m16n8k32 as they lie, without the way through shared and tensor
+// memory that costs the split kernel its start and end.  The order of K within a product is free as long as both operands have the
+// same, so that a lane's fragments are 16 neighbouring bytes: word i of lane q of a row is k = 16 q + 4 i, and two products take words
+// 0, 1 and 2, 3.  Rows of a beyond eight double what every block reads of a, which only small weights have time for.
+// Blocks few per SM have sixteen warps, else eight (eight rows, us: 4 096 x 14 336 11.2 with 16, 15.2 with 8; 10 240 x 8 192 19.7 and
+// 16.1; 4 096 x 4 096 4.5 and 5.8, 57 344 x 8 192 gated 78.9 and 73.0).
+template <int NT, bool WIDE> struct Few {
+  static constexpr int kThreads = WIDE ? 512 : 256, kPerSm = WIDE ? 2 : NT == 1 ? 4 : 3, kTurns = !WIDE && NT == 2 ? 2 : 1;
+};
+
+__device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+template <int OUT, bool SILU, int NT, bool WIDE>
+__global__ void __launch_bounds__(Few<NT, WIDE>::kThreads, Few<NT, WIDE>::kPerSm) few_kernel(const Args g, int n_out) {
+  constexpr int kThreads = Few<NT, WIDE>::kThreads, kTurns = Few<NT, WIDE>::kTurns, kChan = SILU ? 8 : 16, kWarps = kThreads / 32;
+  __shared__ int red[kWarps][16][NT * 8 + 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = lane >> 2, q = lane & 3, n0 = blockIdx.x * kChan;
+  // (past the last channel or row: the last one's again)
+  const int8_t* w0 = g.w + static_cast<size_t>(min(n0 + row, n_out - 1)) * g.K;
+  const int8_t* w1 = g.w + (static_cast<size_t>(SILU ? n_out + min(n0 + row, n_out - 1) : min(n0 + row + 8, n_out - 1))) * g.K;
+  const int8_t* a[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) a[t] = g.a + static_cast<size_t>(min(t * 8 + row, g.M - 1)) * g.K;
+  int acc[NT][4] = {};
+  pdl_trigger();
+  if (q < 2 && warp * 128 < g.K) asm volatile("prefetch.global.L2 [%0];" ::"l"((q ? w1 : w0) + warp * 128));
+  pdl_wait();
+#pragma unroll kTurns
+  for (int k0 = warp * 128; k0 < g.K; k0 += kWarps * 128) {
+    uint4 x[2], y[2], b[2][NT];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int k = k0 + h * 64 + q * 16;
+      const bool in = k < g.K;
+      x[h] = in ? *reinterpret_cast<const uint4*>(w0 + k) : make_uint4(0, 0, 0, 0);
+      y[h] = in ? *reinterpret_cast<const uint4*>(w1 + k) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) b[h][t] = in ? *reinterpret_cast<const uint4*>(a[t] + k) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        mma_s8(acc[t], x[h].x, y[h].x, x[h].y, y[h].y, b[h][t].x, b[h][t].y);
+        mma_s8(acc[t], x[h].z, y[h].z, x[h].w, y[h].w, b[h][t].z, b[h][t].w);
+      }
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    red[warp][row][t * 8 + 2 * q] = acc[t][0];
+    red[warp][row][t * 8 + 2 * q + 1] = acc[t][1];
+    red[warp][row + 8][t * 8 + 2 * q] = acc[t][2];
+    red[warp][row + 8][t * 8 + 2 * q + 1] = acc[t][3];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < kChan * NT * 8; i += kThreads) {
+    const int c = i % kChan, m = i / kChan, n = n0 + c;
+    if (m >= g.M || n >= n_out) continue;
+    float v[2];
+#pragma unroll
+    for (int h = 0; h < (SILU ? 2 : 1); ++h) {
+      int s = 0;
+#pragma unroll
+      for (int p = 0; p < kWarps; ++p) s += red[p][h * 8 + c][m];
       v[h] = scaled(s, g.a_scales[m], g.w_scales[h * n_out + n]);
       if (g.bias) v[h] = __fadd_rn(v[h], load_elem<OUT>(g.bias, h * n_out + n));
     }
@@ -863,13 +940,23 @@ static void launch_split(const Args& g, const Plan& p, cudaStream_t st) {
   B200_CUDA_LAUNCH_CHECK();
 }
 
+template <int OUT, bool SILU, int NT>
+static void launch_few(const Args& g, cudaStream_t st) {
+  const int n_out = SILU ? g.N / 2 : g.N, blocks = (n_out - 1) / (SILU ? 8 : 16) + 1;
+  if (blocks <= 2 * sm_count()) launch_pdl(few_kernel<OUT, SILU, NT, true>, dim3(blocks), dim3(Few<NT, true>::kThreads), 0, st, g, n_out);
+  else launch_pdl(few_kernel<OUT, SILU, NT, false>, dim3(blocks), dim3(Few<NT, false>::kThreads), 0, st, g, n_out);
+  B200_CUDA_LAUNCH_CHECK();
+}
+
 template <int OUT, bool SILU>
 static void launch(const Args& g, cudaStream_t st) {
-  // Up to four rows go without tensor cores (us, against the split kernel): one row of 6 144 x 4 096 5.7 and 8.0, 28 672 x 4 096 gated
-  // 20.5 and 21.9; two rows 6.8 and 8.3, 20.2 and 21.5; four rows 7.2 and 8.3, but 23.0 and 21.5.
+  // What goes without shared and tensor memory, us, against the split kernel: one row of 6 144 x 4 096 5.7 and 8.5, 28 672 x 4 096 gated
+  // 20.3 and 21.5; two rows 6.8 and 8.6, 20.3 and 21.4; eight rows of 4 096 x 4 096 4.5 and 7.0, 6 144 x 4 096 6.5 and 8.3, 28 672 x
+  // 4 096 gated 21.8 and 21.6, 57 344 x 8 192 gated 73.0 and 82.8; sixteen rows 5.7 and 7.2, 6.7 and 8.3, but 4 096 x 14 336 13.7 and 13.6.
   if (g.M == 1) return launch_gemv<OUT, SILU, 1>(g, st);
   if (g.M == 2) return launch_gemv<OUT, SILU, 2>(g, st);
-  if (g.M <= 4 && static_cast<int64_t>(g.N) * g.K <= 100 << 20) return launch_gemv<OUT, SILU, 4>(g, st);
+  if (g.M <= 8) return launch_few<OUT, SILU, 1>(g, st);
+  if (g.M <= 16 && static_cast<int64_t>(g.N) * g.K <= 32 << 20) return launch_few<OUT, SILU, 2>(g, st);
   const Plan p = plan(g);
   if (p.group == 0) launch_pairs<OUT, SILU>(g, p.T, st);
   else if (p.group == 1) launch_split<OUT, SILU, 1>(g, p, st);
