@@ -112,7 +112,8 @@ static_assert(kPairSmem <= 227 * 1024, "shared memory budget");
 
 struct PairArgs {
   Args g;
-  int n_out, KB, bn, tiles_m, tiles_n, group_m, wide;
+  int n_out, KB, bn, tiles_m, tiles_n, group_m;
+  int wide;            // results' rows begin on 16 bytes (2), on 4 (1) or anywhere
   int* err;
 };
 
@@ -240,10 +241,10 @@ pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CU
       __syncwarp();
       tc_fence_after();
       const uint32_t src = tmem + lanes + buf * 256;
-      // the staged rows' bytes: `count` columns from c on
-      auto store = [&](int c, int count) {
+      // the staged rows' 64 bytes from column c on
+      auto store = [&](int c) {
         __syncwarp();
-        if (a.wide) {
+        if (a.wide == 2) {
           const int sub = (lane & 3) * 16, col = n0 + c + sub / kElem;
           if (col < a.n_out) {
 #pragma unroll
@@ -254,11 +255,31 @@ pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CU
                     *reinterpret_cast<const uint4*>(stage + rw * kPitch + sub);
             }
           }
-        } else if (lane < count && n0 + c + lane < a.n_out) {
-          for (int rw = 0; rw < 32 && rw < rows; ++rw) {
-            const size_t at = static_cast<size_t>(row0 + rw) * a.n_out + n0 + c + lane;
-            if constexpr (OUT == kF32) static_cast<float*>(a.g.c)[at] = *reinterpret_cast<const float*>(stage + rw * kPitch + lane * 4);
-            else static_cast<uint16_t*>(a.g.c)[at] = *reinterpret_cast<const uint16_t*>(stage + rw * kPitch + lane * 2);
+        } else if (OUT == kF32 || a.wide == 0) {       // results of any pitch: element by element, of fp32 two rows at once
+          const int col = OUT == kF32 ? lane & 15 : lane, first = OUT == kF32 ? lane >> 4 : 0;
+          if (n0 + c + col < a.n_out) {
+            uint8_t* dst = static_cast<uint8_t*>(a.g.c) + (static_cast<size_t>(row0 + first) * a.n_out + n0 + c + col) * kElem;
+            const uint8_t* src = stage + first * kPitch + col * kElem;
+#pragma unroll 8
+            for (int i = 0; i < (OUT == kF32 ? 16 : 32); ++i) {
+              constexpr int kRows = OUT == kF32 ? 2 : 1;
+              if (first + i * kRows < rows) {
+                if constexpr (OUT == kF32) *reinterpret_cast<float*>(dst) = *reinterpret_cast<const float*>(src + i * 2 * kPitch);
+                else *reinterpret_cast<uint16_t*>(dst) = *reinterpret_cast<const uint16_t*>(src + i * kPitch);
+              }
+              dst += static_cast<size_t>(a.n_out) * kElem * kRows;
+            }
+          }
+        } else {                                       // 16 bits of an even pitch: two neighbours, two rows at once
+          const int col = (lane & 15) * 2, first = lane >> 4;
+          if (n0 + c + col < a.n_out) {
+            uint8_t* dst = static_cast<uint8_t*>(a.g.c) + (static_cast<size_t>(row0 + first) * a.n_out + n0 + c + col) * kElem;
+            const uint8_t* src = stage + first * kPitch + col * kElem;
+#pragma unroll 8
+            for (int i = 0; i < 16; ++i) {
+              if (first + i * 2 < rows) *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(src + i * 2 * kPitch);
+              dst += static_cast<size_t>(a.n_out) * kElem * 2;
+            }
           }
         }
         __syncwarp();
@@ -302,7 +323,7 @@ pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CU
               for (int i = 0; i < 16; i += 4)
                 *reinterpret_cast<uint4*>(stage + lane * kPitch + i * 4) =
                     make_uint4(v[hf * 16 + i], v[hf * 16 + i + 1], v[hf * 16 + i + 2], v[hf * 16 + i + 3]);
-              store(c + hf * 16, 16);
+              store(c + hf * 16);
             }
           } else {
 #pragma unroll
@@ -312,7 +333,7 @@ pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CU
               for (int e = 0; e < 4; ++e) h[e] = pack16x2<OUT == kBF16>(__uint_as_float(v[i + 2 * e]), __uint_as_float(v[i + 2 * e + 1]));
               *reinterpret_cast<uint4*>(stage + lane * kPitch + i * 2) = make_uint4(h[0], h[1], h[2], h[3]);
             }
-            store(c, 32);
+            store(c);
           }
         }
       }
@@ -786,7 +807,8 @@ static void launch_pairs(const Args& g, int bn, cudaStream_t st) {
   a.tiles_m = g.M / 256 + (g.M % 256 != 0);
   a.tiles_n = (a.n_out + (SILU ? bn / 2 : bn) - 1) / (SILU ? bn / 2 : bn);
   a.group_m = 16;
-  a.wide = ((reinterpret_cast<uintptr_t>(g.c) | (static_cast<uintptr_t>(a.n_out) * kElem)) & 15) == 0;
+  const uintptr_t places = reinterpret_cast<uintptr_t>(g.c) | (static_cast<uintptr_t>(a.n_out) * kElem);
+  a.wide = (places & 15) == 0 ? 2 : (places & 3) == 0 ? 1 : 0;
   a.err = wait_error_flag();
   CUtensorMap amap, wmap;
   if (!map_rows(&amap, g.a, g.M, g.K, 128) || !map_rows(&wmap, g.w, g.N, g.K, bn / 2) || !a.err) {
