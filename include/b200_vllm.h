@@ -138,7 +138,7 @@ void b200_dense_gemm_ex(const void* a, const void* w, const void* bias, void* c,
 /* ------------------------------------------------- linear layers in 8-bit integers (weights and activations)
  * Rows to codes, a scale per row (the symmetric form of 8-bit checkpoints): out int8 [rows, width], scales fp32 [rows],
  * value = code * scale, codes in [-127, 127].  q = round(127 t / max|t|), ties to even, exactly, with t = x, or x * weight behind
- * an RMS norm (1 / rms is part of the scale only): codes are the same whatever the launch.  Any width up to 2^30.  A row of zeros
+ * an RMS norm (1 / rms is part of the scale only): codes are the same whatever the launch.  Widths and rows up to 2^30.  A row of zeros
  * has scale 0; a row with a NaN or an infinity has scale NaN and codes 0, so that what is computed from it is NaN.
  * add_rmsnorm: residual += x first (rounded to 16 bits, as b200_add_rmsnorm_f16), then the norm of the residual.
  * quant_rows also makes the weights' codes, a scale per output channel.                                            */
@@ -153,7 +153,7 @@ void b200_add_rmsnorm_i8_bf16(void* out, float* scales, void* residual, const vo
 void b200_quant_rows_i8_f16(void* out, float* scales, const void* x, int32_t rows, int32_t width, int64_t stream);
 void b200_quant_rows_i8_bf16(void* out, float* scales, const void* x, int32_t rows, int32_t width, int64_t stream);
 /* c[m, n] = (sum_k a[m, k] w[n, k]) * a_scales[m] * w_scales[n] (+ bias[n]): int8 a [m, k] and w [n, k], 16-byte aligned, k a
- * multiple of 16 and at most 131056 (int32 sums stay exact for any codes), any m and n; fp32 epilogue, one rounding to the type
+ * multiple of 16 and at most 131056 (int32 sums stay exact for any codes), m and n up to 2^30; fp32 epilogue, one rounding to the type
  * of the suffix, which is bias's type too (bias may be NULL).  epilogue B200_EPI_SILU_MUL: w = gate rows, then as many up rows,
  * c [m, n / 2] = silu(gate) * up of the fp32 values.  No workspace; results do not depend on the launch's shape.        */
 void b200_gemm_i8_f16(const void* a, const float* a_scales, const void* w, const float* w_scales, const void* bias,

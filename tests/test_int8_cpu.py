@@ -33,6 +33,9 @@ def test_rows_refuse(lib, suffix):
     _refused(lib, lambda: f("quant_rows")(A, A, A, 2, 0, 0), b"quant_rows_i8")
     _refused(lib, lambda: f("quant_rows")(A, A, A, 2, 2 ** 30 + 1, 0), b"quant_rows_i8")
     _refused(lib, lambda: f("quant_rows")(A, None, A, 2, 8, 0), b"quant_rows_i8")
+    _refused(lib, lambda: f("quant_rows")(A, A, A, 2 ** 30 + 1, 8, 0), b"quant_rows_i8")
+    _refused(lib, lambda: f("rmsnorm")(A, A, A, A, 2 ** 30 + 1, 64, eps, 0), b"rmsnorm_i8")
+    _refused(lib, lambda: f("add_rmsnorm")(A, A, A, A, A, 2 ** 30 + 1, 64, eps, 0), b"add_rmsnorm_i8")
     f("quant_rows")(None, None, None, 0, 8, 0)                           # no rows: nothing to do, nothing to refuse
     assert lib.b200_last_error() == 0
 
@@ -46,7 +49,9 @@ def test_gemm_refuses(lib, suffix):
         _refused(lib, lambda: f(*p, 4, 64, 64, 0, 0), b"gemm_i8: bad arguments")
     ok = [A, A, A, A, None, A]
     for m, n, k, epi, words in ((4, 0, 64, 0, b"bad arguments"), (4, 64, 0, 0, b"bad arguments"), (4, 64, 72, 0, b"multiple of 16"),
-                                (4, 64, 131072, 0, b"at most 131056"), (4, 63, 64, 1, b"odd number"), (4, 64, 64, 2, b"unknown epilogue")):
+                                (4, 64, 131072, 0, b"at most 131056"),
+                                (2 ** 30 + 1, 64, 64, 0, b"at most 2^30"), (4, 2 ** 30 + 1, 64, 0, b"at most 2^30"),
+                                (4, 63, 64, 1, b"odd number"), (4, 64, 64, 2, b"unknown epilogue")):
         _refused(lib, lambda: f(*ok, m, n, k, epi, 0), words)
     _refused(lib, lambda: f(ODD, A, A, A, None, A, 4, 64, 64, 0, 0), b"16-byte aligned")
     _refused(lib, lambda: f(A, A, ODD, A, None, A, 4, 64, 64, 0, 0), b"16-byte aligned")
@@ -105,3 +110,14 @@ def test_wrappers_refuse_products(ops):
             call()
     with pytest.raises(TypeError):
         ops.gemm_i8(q, s, w, t, dtype=torch.float64)
+
+
+@pytest.mark.parametrize("rows,width", [(2 ** 32 + 3, 1), (1, 2 ** 32 + 16), (2 ** 30 + 1, 16)])
+def test_wrappers_refuse_what_32_bits_do_not_count(ops, rows, width):
+    make = lambda *shape, dtype=torch.float16: torch.empty(shape, dtype=dtype, device="meta")        # noqa: E731
+    x, w, q = make(rows, width), make(width), make(rows, width, dtype=torch.int8)
+    one, s1, s = make(1, width, dtype=torch.int8), make(1, dtype=torch.float32), make(rows, dtype=torch.float32)
+    for call in (lambda: ops.quant_rows_i8(x), lambda: ops.rmsnorm_i8(x, w, 1e-5), lambda: ops.add_rmsnorm_i8(x, x, w, 1e-5),
+                 lambda: ops.gemm_i8(q, s, one, s1), lambda: ops.gemm_i8(one, s1, q, s)):
+        with pytest.raises(ValueError, match="2\\^30"):
+            call()

@@ -20,6 +20,7 @@ namespace b200 {
 namespace gemm8 {
 
 constexpr int kMaxK = 131056;        // 2^31 / 128^2 = 131072 products of the largest size overflow; the multiple of 16 below
+constexpr int kMaxRows = 1 << 30;    // rows and channels are counted in 32 bits, a tile past the end
 constexpr int kBK = 128;             // K of a stage: one 128-byte swizzle row, four products of 32
 constexpr uint32_t kHiSw128 = (1024 >> 4) | (1u << 14) | (2u << 29);
 
@@ -1015,6 +1016,7 @@ template <int OUT>
 static void gemm(const Args& g, int epilogue, int64_t stream) {
   const bool silu = epilogue == B200_EPI_SILU_MUL;
   B200_CHECK_ARG(g.a && g.a_scales && g.w && g.w_scales && g.c && g.N > 0 && g.K > 0, "gemm_i8: bad arguments");
+  B200_CHECK_ARG(g.M <= kMaxRows && g.N <= kMaxRows, "gemm_i8: m and n can be at most 2^30");
   B200_CHECK_ARG(g.K % 16 == 0 && g.K <= kMaxK, "gemm_i8: k must be a multiple of 16 and at most 131056");
   B200_CHECK_ARG(((reinterpret_cast<uintptr_t>(g.a) | reinterpret_cast<uintptr_t>(g.w)) & 15) == 0,
                  "gemm_i8: rows and weights must be 16-byte aligned");

@@ -24,7 +24,7 @@ namespace b200 {
 namespace rows8 {
 
 constexpr int kWarpRows = 8;        // rows of a block where each warp has one
-constexpr int kMaxWidth = 1 << 30;  // columns are counted in 32 bits
+constexpr int kMaxWidth = 1 << 30, kMaxRows = 1 << 30;      // columns and rows are counted in 32 bits, a block or a tile past the end
 
 struct Args {
   int8_t* out;
@@ -380,6 +380,8 @@ static void launch(const Args& a, cudaStream_t st) {
   go(rows_i8_kernel<BF, NORM, ADD, LAY, false, 8>, a.rows, threads());
 }
 
+static bool counted(int rows, int width) { return rows <= kMaxRows && width > 0 && width <= kMaxWidth; }
+
 template <bool BF, bool NORM, bool ADD>
 static void rows_i8(void* out, float* scales, void* residual, const void* x, const void* w, int rows, int width, float eps,
                     int64_t stream) {
@@ -401,21 +403,22 @@ static void rows_i8(void* out, float* scales, void* residual, const void* x, con
                                            int32_t hidden, float eps, int64_t stream) {                                        \
     using namespace b200;                                                                                                      \
     if (num_tokens <= 0) return;                                                                                               \
-    B200_CHECK_ARG(out && scales && x && weight && hidden > 0 && hidden <= rows8::kMaxWidth, "rmsnorm_i8: bad arguments");     \
+    B200_CHECK_ARG(out && scales && x && weight && rows8::counted(num_tokens, hidden), "rmsnorm_i8: bad arguments");           \
     rows8::rows_i8<BF, true, false>(out, scales, nullptr, x, weight, num_tokens, hidden, eps, stream);                         \
   }                                                                                                                            \
   extern "C" void b200_add_rmsnorm_i8_##SUFFIX(void* out, float* scales, void* residual, const void* x, const void* weight,    \
                                                int32_t num_tokens, int32_t hidden, float eps, int64_t stream) {                \
     using namespace b200;                                                                                                      \
     if (num_tokens <= 0) return;                                                                                               \
-    B200_CHECK_ARG(out && scales && residual && x && weight && hidden > 0 && hidden <= rows8::kMaxWidth, "add_rmsnorm_i8: bad arguments");\
+    B200_CHECK_ARG(out && scales && residual && x && weight && rows8::counted(num_tokens, hidden),                           \
+                   "add_rmsnorm_i8: bad arguments");                                                                           \
     rows8::rows_i8<BF, true, true>(out, scales, residual, x, weight, num_tokens, hidden, eps, stream);                         \
   }                                                                                                                            \
   extern "C" void b200_quant_rows_i8_##SUFFIX(void* out, float* scales, const void* x, int32_t rows, int32_t width,            \
                                               int64_t stream) {                                                                \
     using namespace b200;                                                                                                      \
     if (rows <= 0) return;                                                                                                     \
-    B200_CHECK_ARG(out && scales && x && width > 0 && width <= rows8::kMaxWidth, "quant_rows_i8: bad arguments");              \
+    B200_CHECK_ARG(out && scales && x && rows8::counted(rows, width), "quant_rows_i8: bad arguments");                         \
     rows8::rows_i8<BF, false, false>(out, scales, nullptr, x, nullptr, rows, width, 0.f, stream);                              \
   }
 B200_ROWS_I8(f16, false)

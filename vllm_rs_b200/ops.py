@@ -150,6 +150,14 @@ def _refuse(t, shape, dtype, what):
     raise ValueError(f"{what} must be {tuple(shape)} in {dtype}, got {tuple(t.shape)} in {t.dtype}")
 
 
+_I8_MOST = 1 << 30           # rows, channels and widths that the kernels count (entry points take 32 bits: a longer one would wrap)
+
+
+def _i8_count(*ns):
+    if max(ns) > _I8_MOST:
+        raise ValueError(f"sizes up to 2^30 are supported, got {ns}")
+
+
 def _i8_results(x, out, scales):
     """The tensors of the codes and of the scales of rows x, checked where they are given."""
     shape = x.shape
@@ -185,6 +193,7 @@ def quant_rows_i8(x, out=None, scales=None):
         raise ValueError(f"rows must be [rows, width], got {tuple(x.shape)}")
     out, scales = _i8_results(x, out, scales)
     rows, width = x.shape
+    _i8_count(rows, width)
     fn(out.data_ptr(), scales.data_ptr(), x.data_ptr(), rows, width, stream)
     _lib.check()
     return out, scales
@@ -197,6 +206,7 @@ def rmsnorm_i8(x, w, eps, out=None, scales=None):
     _i8_norm_checks(x, w)
     out, scales = _i8_results(x, out, scales)
     rows, width = x.shape
+    _i8_count(rows, width)
     fn(out.data_ptr(), scales.data_ptr(), x.data_ptr(), w.data_ptr(), rows, width, eps, stream)
     _lib.check()
     return out, scales
@@ -211,6 +221,7 @@ def add_rmsnorm_i8(residual, x, w, eps, out=None, scales=None):
         _refuse(residual, x.shape, x.dtype, "residual")
     out, scales = _i8_results(x, out, scales)
     rows, width = x.shape
+    _i8_count(rows, width)
     fn(out.data_ptr(), scales.data_ptr(), residual.data_ptr(), x.data_ptr(), w.data_ptr(), rows, width, eps, stream)
     _lib.check()
     return out, scales
@@ -227,6 +238,7 @@ def gemm_i8(x, x_scales, w_nk, w_scales, bias=None, epilogue=EPI_NONE, dtype=tor
                          f"{tuple(w_nk.shape)} in {w_nk.dtype}")
     m, k = x.shape
     n = w_nk.shape[0]
+    _i8_count(m, n, k)
     if x_scales.shape != (m,) or x_scales.dtype != torch.float32:
         _refuse(x_scales, (m,), torch.float32, "rows' scales")
     if w_scales.shape != (n,) or w_scales.dtype != torch.float32:
