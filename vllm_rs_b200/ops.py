@@ -153,9 +153,8 @@ def _refuse(t, shape, dtype, what):
 _I8_MOST = 1 << 30           # rows, channels and widths that the kernels count (entry points take 32 bits: a longer one would wrap)
 
 
-def _i8_count(*ns):
-    if max(ns) > _I8_MOST:
-        raise ValueError(f"sizes up to 2^30 are supported, got {ns}")
+def _i8_too_long(*sizes):
+    raise ValueError(f"sizes up to 2^30 are supported, got {sizes}")
 
 
 def _i8_results(x, out, scales):
@@ -193,7 +192,8 @@ def quant_rows_i8(x, out=None, scales=None):
         raise ValueError(f"rows must be [rows, width], got {tuple(x.shape)}")
     out, scales = _i8_results(x, out, scales)
     rows, width = x.shape
-    _i8_count(rows, width)
+    if rows > _I8_MOST or width > _I8_MOST:
+        _i8_too_long(rows, width)
     fn(out.data_ptr(), scales.data_ptr(), x.data_ptr(), rows, width, stream)
     _lib.check()
     return out, scales
@@ -206,7 +206,8 @@ def rmsnorm_i8(x, w, eps, out=None, scales=None):
     _i8_norm_checks(x, w)
     out, scales = _i8_results(x, out, scales)
     rows, width = x.shape
-    _i8_count(rows, width)
+    if rows > _I8_MOST or width > _I8_MOST:
+        _i8_too_long(rows, width)
     fn(out.data_ptr(), scales.data_ptr(), x.data_ptr(), w.data_ptr(), rows, width, eps, stream)
     _lib.check()
     return out, scales
@@ -221,7 +222,8 @@ def add_rmsnorm_i8(residual, x, w, eps, out=None, scales=None):
         _refuse(residual, x.shape, x.dtype, "residual")
     out, scales = _i8_results(x, out, scales)
     rows, width = x.shape
-    _i8_count(rows, width)
+    if rows > _I8_MOST or width > _I8_MOST:
+        _i8_too_long(rows, width)
     fn(out.data_ptr(), scales.data_ptr(), residual.data_ptr(), x.data_ptr(), w.data_ptr(), rows, width, eps, stream)
     _lib.check()
     return out, scales
@@ -238,7 +240,8 @@ def gemm_i8(x, x_scales, w_nk, w_scales, bias=None, epilogue=EPI_NONE, dtype=tor
                          f"{tuple(w_nk.shape)} in {w_nk.dtype}")
     m, k = x.shape
     n = w_nk.shape[0]
-    _i8_count(m, n, k)
+    if m > _I8_MOST or n > _I8_MOST or k > _I8_MOST:
+        _i8_too_long(m, n, k)
     if x_scales.shape != (m,) or x_scales.dtype != torch.float32:
         _refuse(x_scales, (m,), torch.float32, "rows' scales")
     if w_scales.shape != (n,) or w_scales.dtype != torch.float32:
