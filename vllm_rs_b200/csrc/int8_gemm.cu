@@ -874,16 +874,19 @@ static_assert(smem_floor(512) <= kMaxSmem && smem_floor(256) <= 113 * 1024, "wha
 // Blocks of the split kernel that an SM holds take all of its shared memory or half of it.
 constexpr int kWholeSm = 226 * 1024, kHalfSm = 113 * 1024;
 
-// How many clusters of 1 to 8 of them the chip holds at once (of eight whole SMs: 15, since few groups of SMs have 16 to give).
+// How many clusters of 1 to 8 of them the chip holds at once (of eight whole SMs: 15, since few groups of SMs have 16 to give).  What
+// is asked about has the split kernel's threads but no tensor memory: of kernels that allocate some the runtime counts one block per
+// SM, whatever their sizes, while two run there at once (seen by their SMs and times; `smem_floor` keeps them within the 512 columns).
+__global__ void __launch_bounds__(kSplitThreads) split_shape() {}
+
 struct Room {
   int whole[8], half[8];
   Room() {
-    const auto kern = split_kernel<kF16, false, 1>;
-    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+    cudaFuncSetAttribute(split_shape, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
     for (int c = 1; c <= 8; ++c) {
       const dim3 grid(sm_count() / c * c);
-      const int w = max_active_clusters(kern, grid, dim3(kSplitThreads), kWholeSm, dim3(c));
-      const int h = max_active_clusters(kern, grid, dim3(kSplitThreads), kHalfSm, dim3(c));
+      const int w = max_active_clusters(split_shape, grid, dim3(kSplitThreads), kWholeSm, dim3(c));
+      const int h = max_active_clusters(split_shape, grid, dim3(kSplitThreads), kHalfSm, dim3(c));
       whole[c - 1] = w > 0 ? w : sm_count() / c;
       half[c - 1] = h > 0 ? h : 2 * sm_count() / c;
     }
@@ -900,12 +903,14 @@ struct Plan {
   int group, T, splits, smem;
 };
 
-// The estimates (us) are fits to 311 shapes (8 to 4 096 rows, N and K from 256 to 28 672), each measured in every form; the form taken
-// costs 1 % more than the best one in the mean, a sixth at most.  A block of K takes as long as the tensor core, the L2 (7.8 ns
-// a KB) or the memory's answer over the stages that wait for it; weights come at 7.4 TB/s at best; an epilogue 12 ns a row; a
-// meeting of parts 0.6 us where their sums have a place of their own, else 1.7, and 0.36 for each further part.  What the choice is
-// worth, us: 257 rows of 4 096 x 14 336 pairs 42, one part 28, two parts 18.7 - 20.1, four of half an SM 24; 1 003 of 10 240 x
-// 8 192 pairs 62.6 (256 wide 64.3), split 72.5.
+// The estimates (us) are fits to 437 shapes (16 to 4 096 rows, N from 256 to 128 256, K from 512 to 28 672), each measured in every form;
+// the form taken costs 0.6 % more than the best one in the mean, a seventh at most (rows so few that start and end are all).  A block
+// of K takes as long as the tensor core, the L2 (7.1 ns a KB), the memory's answer over the stages that wait for it, or what one SM
+// takes in from memory (0.18 us for 128 weight rows: few SMs do not fetch at the chip's rate); weights come at 8.4 TB/s at best (the L2
+// held some); an epilogue 13 ns a row, another turn of blocks 3.5 us; a meeting of parts 0.7 us where their sums have a place of their
+// own, else 1.6, and 0.3 for each further part.  What the choice is worth, us: 257 rows of 4 096 x 14 336 pairs 42, one part 28, two
+// parts 18.7 - 20.1, four of half an SM 24; 1 003 of 10 240 x 8 192 pairs 62.6 (256 wide 64.3), split 72.5; 32 of 8 192 x 28 672 one part
+// 46, two 38; 128 of 20 480 x 8 192 one part 35.7, two 45.4.
 static Plan plan(const Args& g) {
   static const Room room;
   const int KB = (g.K + kBK - 1) / kBK;
@@ -920,8 +925,8 @@ static Plan plan(const Args& g) {
   if (g.M > 128)
     for (int bn = 64; bn <= 256; bn += 64) {
       const int64_t tiles = (static_cast<int64_t>(g.M) + 255) / 256 * ((g.N - 1) / bn + 1), pairs = sm_count() / 2;
-      const float block = (128 + bn / 2) * kBK * 9.15e-6f;
-      offer(2.19f + static_cast<float>((tiles + pairs - 1) / pairs) * (KB * block + 1.11f) + bn * 9.4e-3f, Plan{0, bn, 1, 0});
+      const float block = (128 + bn / 2) * kBK * 10.23e-6f;
+      offer(2.22f + static_cast<float>((tiles + pairs - 1) / pairs) * (KB * block + 0.91f) + bn * 6.2e-3f, Plan{0, bn, 1, 0});
     }
   if (g.M <= 1536)
     for (int parts = 1; parts <= 5; ++parts) {
@@ -937,11 +942,11 @@ static Plan plan(const Args& g) {
             if (!whole && (T > 256 || sums_bytes(T, splits) > kHalfSm - kSplitFixed)) continue;      // (two blocks share tensor memory, too)
             const int share = whole ? 1 : 2, smem = whole ? kWholeSm : kHalfSm;
             const int64_t rounds = whole ? 1 : (tiles + room.half[c] - 1) / room.half[c];
-            const int stages = std::min((smem - kSplitFixed) / stage, kMaxStages);
-            const float block = std::max({share * T * 1.21e-3f, share * stage * 7.63e-6f, 1.44f / stages});
-            const float stream = std::max(static_cast<float>(g.N) * g.K * 0.136e-6f, rounds * ((KB + splits - 1) / splits) * block);
-            offer(1.59f + stream + rounds * (share * T * 12.2e-3f + 0.88f) - 0.88f +
-                      (splits > 1 ? (T > 64 ? 1.65f : 0.53f) + 0.36f * (splits - 1) : 0.f) + (group == 2 ? 0.64f : 0.f),
+            const int own = T <= 64 ? sums_bytes(T, splits) : 0, stages = std::max(std::min((smem - kSplitFixed - own) / stage, kMaxStages), 1);
+            const float block = std::max({share * T * 1.28e-3f, share * stage * 7.1e-6f, 1.54f / stages, share * 0.184f});
+            const float stream = std::max(static_cast<float>(g.N) * g.K * 0.1187e-6f, rounds * ((KB + splits - 1) / splits) * block);
+            offer(1.63f + stream + rounds * (share * T * 13.35e-3f + 3.51f) - 3.51f +
+                      (splits > 1 ? (T > 64 ? 1.6f : 0.74f) + 0.32f * (splits - 1) : 0.f) + (group == 2 ? 0.59f : 0.f),
                   Plan{group, T, splits, smem});
           }
         }
