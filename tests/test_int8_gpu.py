@@ -217,7 +217,10 @@ CUTS = [(3, 130, 272), (3, 130, 2064), (3, 130, 4096), (3, 130, 8192), (3, 4096,
         (129, 3000, 8192), (200, 1000, 8192), (200, 3000, 4096), (257, 1536, 8192), (257, 10240, 272), (257, 10240, 1024),
         (300, 1536, 4096), (300, 10240, 272), (300, 10240, 1024), (333, 2048, 8192), (500, 5000, 1024), (500, 10240, 272),
         (600, 10240, 272), (700, 5000, 272), (700, 8192, 272), (900, 130, 272), (900, 130, 4096), (900, 130, 8192),
-        (900, 1000, 4096), (900, 1536, 272), (900, 1536, 1024), (900, 1536, 4096), (900, 5000, 272), (900, 5000, 1024)]
+        (900, 1000, 4096), (900, 1536, 272), (900, 1536, 1024), (900, 1536, 4096), (900, 5000, 272), (900, 5000, 1024),
+        (17, 34, 8544), (17, 36, 4160), (18, 4768, 1520), (17, 9572, 6192), (40, 24000, 1040), (41, 9566, 9120), (91, 32, 7088),
+        (203, 10144, 8400), (645, 9416, 1056), (1216, 1816, 6928), (1281, 1036, 9360), (1287, 638, 7184), (1291, 36, 6768),
+        (1296, 800, 5312), (1316, 70, 6240), (1322, 734, 6976), (1394, 502, 5968)]
 
 
 @pytest.mark.parametrize("m,n,k", CUTS)
@@ -227,6 +230,19 @@ def test_products_however_cut(ops, m, n, k):
     _check_product(ops.gemm_i8(a, sa, w, sw, dtype=F32), a, sa, w, sw, None, F32)
     sw = sw * 4
     _check_product(ops.gemm_i8(a, sa, w, sw, bias=bias, dtype=BF16, epilogue=ops.EPI_SILU_MUL), a, sa, w, sw, bias, BF16, True)
+
+
+# one row and two, in blocks of four warps and of eight, the last of them full and not
+@pytest.mark.parametrize("silu", [False, True], ids=["plain", "gated"])
+@pytest.mark.parametrize("n,k", [(2, 16), (34, 8208), (3500, 528), (3560, 528), (5120, 5120), (6002, 1040), (7102, 2064), (7110, 2064),
+                                 (8190, 2576), (10654, 2064), (10660, 2064), (24002, 272)])
+def test_single_rows(ops, n, k, silu):
+    a, sa, w, sw, bias = (t.cuda() for t in _case(2, n, k, BF16, True))
+    for m in (1, 2):
+        out = torch.full((m + 2, n // 2 if silu else n), 7.0, dtype=BF16, device="cuda")
+        y = ops.gemm_i8(a[:m], sa[:m], w, sw, bias=bias, dtype=BF16, epilogue=int(silu), out=out[1:m + 1])
+        _check_product(y, a[:m], sa[:m], w, sw, bias, BF16, silu)
+        assert bool((out[0] == 7).all()) and bool((out[-1] == 7).all())
 
 
 @pytest.mark.parametrize("m", [1, 32, 130, 300])

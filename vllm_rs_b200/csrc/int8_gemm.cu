@@ -646,20 +646,16 @@ split_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
 }
 
 // ------------------------------------------------------------------ one row or two
-// A block has `Rows` weight rows (gated: half of them gate rows, half the up rows of the same channels); its warps take 512 of K in turn,
-// `Rows` 16-byte loads a lane at once, four products per dp4a.  Blocks are small and many per SM, so that enough loads are under way
-// and the last ones end together (one row of 4 096 x 14 336, us: 256 threads with 4 rows, 8 blocks per SM 10.5; with 8 rows, 4 blocks
-// 10.9; 128 threads with 8 rows 12.5.  Two rows: 128 threads with 8 rows 10.4, 256 with 8 13.3, with 4 13.0).  One row of which the
-// last turn of eight warps would leave more than an eighth idle has four warps a block (256 and 128 threads: 5 120 x 5 120 8.3 and 6.3,
-// 27 648 x 5 120 gated 26.3 and 22.8, 5 120 x 13 824 15.6 and 13.8, 151 936 x 2 048 55.9 and 45.4; but 4 096 x 4 096 3.9 and 4.4,
-// 4 608 x 3 584 3.8 and 4.4, 3 584 x 18 944 13.4 and 16.0).
-template <int MT, int THREADS> struct Gemv {
-  static constexpr int kRows = MT == 1 ? 4 : 8, kPerSm = MT == 1 ? 2048 / THREADS : 5;
+// A block has `kRows` weight rows (gated: half of them gate rows, half the up rows of the same channels); its warps take 512 of K in
+// turn, `kRows` 16-byte loads a lane at once, four products per dp4a.  Blocks are small and many per SM, so that enough loads are under
+// way and the last ones end together: four warps, or eight (WIDE) as `wide_rows` says.
+template <int MT, bool WIDE> struct Gemv {
+  static constexpr int kThreads = WIDE ? 256 : 128, kRows = WIDE ? 6 : 8, kPerSm = WIDE ? 4 : MT == 1 ? 6 : 5;
 };
 
-template <int OUT, bool SILU, int MT, int THREADS>
-__global__ void __launch_bounds__(THREADS, Gemv<MT, THREADS>::kPerSm) gemv_kernel(const Args g, int n_out) {
-  constexpr int kGemvThreads = THREADS, kGemvRows = Gemv<MT, THREADS>::kRows;
+template <int OUT, bool SILU, int MT, bool WIDE>
+__global__ void __launch_bounds__(Gemv<MT, WIDE>::kThreads, Gemv<MT, WIDE>::kPerSm) gemv_kernel(const Args g, int n_out) {
+  constexpr int kGemvThreads = Gemv<MT, WIDE>::kThreads, kGemvRows = Gemv<MT, WIDE>::kRows;
   constexpr int kChan = SILU ? kGemvRows / 2 : kGemvRows;
   __shared__ int red[kGemvThreads / 32][kGemvRows * MT];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n0 = blockIdx.x * kChan;
@@ -859,12 +855,22 @@ static void launch_pairs(const Args& g, int bn, cudaStream_t st) {
   B200_CUDA_LAUNCH_CHECK();
 }
 
-template <int OUT, bool SILU, int MT, int THREADS>
+template <int OUT, bool SILU, int MT, bool WIDE>
 static void launch_gemv(const Args& g, cudaStream_t st) {
-  constexpr int kChan = SILU ? Gemv<MT, THREADS>::kRows / 2 : Gemv<MT, THREADS>::kRows;
+  constexpr int kChan = SILU ? Gemv<MT, WIDE>::kRows / 2 : Gemv<MT, WIDE>::kRows;
   const int n_out = SILU ? g.N / 2 : g.N;
-  launch_pdl(gemv_kernel<OUT, SILU, MT, THREADS>, dim3((n_out - 1) / kChan + 1), dim3(THREADS), 0, st, g, n_out);
+  launch_pdl(gemv_kernel<OUT, SILU, MT, WIDE>, dim3((n_out - 1) / kChan + 1), dim3(Gemv<MT, WIDE>::kThreads), 0, st, g, n_out);
   B200_CUDA_LAUNCH_CHECK();
+}
+
+// One row: blocks of eight warps where those of four would be too few to fill half the chip, or would leave the second of two turns
+// mostly empty.  us, four warps and eight: 4 096 x 14 336 10.2 and 11.6, 6 144 x 4 096 4.9 and 5.6, 28 672 x 4 096 18.9 and 20.0,
+// 5 120 x 5 120 5.5 and 6.8, 151 936 x 2 048 45.5 and 65.9, 8 192 x 2 048 4.4 and 4.9; but 1 024 x 8 192 4.6 and 3.4, 2 560 x 6 144 4.4
+// and 4.0, 8 192 x 4 096 7.6 and 6.7, 10 240 x 8 192 15.1 and 13.7, 8 192 x 28 672 39.3 and 35.9.  In later turns, 14 336 to 57 344
+// channels, the two are within 5 % at K from 7 168.
+static bool wide_rows(const Args& g) {
+  const int64_t blocks = (g.N - 1) / Gemv<1, false>::kRows + 1, at_once = static_cast<int64_t>(Gemv<1, false>::kPerSm) * sm_count();
+  return blocks * 2 < at_once || (g.K > 2048 && blocks > at_once && blocks * 2 < at_once * 3);
 }
 
 // Shared memory that a block asks for at least, so that the blocks on an SM never want more tensor memory together than there is: a
@@ -1010,11 +1016,8 @@ static void launch(const Args& g, cudaStream_t st) {
   // What goes without shared and tensor memory, us, against the split kernel: one row of 6 144 x 4 096 5.7 and 8.5, 28 672 x 4 096 gated
   // 20.3 and 21.5; two rows 6.8 and 8.6, 20.3 and 21.4; eight rows of 4 096 x 4 096 4.5 and 7.0, 6 144 x 4 096 6.5 and 8.3, 28 672 x
   // 4 096 gated 21.8 and 21.6, 57 344 x 8 192 gated 73.0 and 82.8; sixteen rows 5.7 and 7.2, 6.7 and 8.3, but 4 096 x 14 336 13.7 and 13.6.
-  if (g.M == 1) {
-    const int turn = 256 * 16, idle = (turn - g.K % turn) % turn;
-    return idle * 8 > g.K + idle ? launch_gemv<OUT, SILU, 1, 128>(g, st) : launch_gemv<OUT, SILU, 1, 256>(g, st);
-  }
-  if (g.M == 2) return launch_gemv<OUT, SILU, 2, 128>(g, st);
+  if (g.M == 1) return wide_rows(g) ? launch_gemv<OUT, SILU, 1, true>(g, st) : launch_gemv<OUT, SILU, 1, false>(g, st);
+  if (g.M == 2) return launch_gemv<OUT, SILU, 2, false>(g, st);
   if (g.M <= 8) return launch_few<OUT, SILU, 1>(g, st);
   if (g.M <= 16 && static_cast<int64_t>(g.N) * g.K <= 32 << 20) return launch_few<OUT, SILU, 2>(g, st);
   const Plan p = plan(g);
