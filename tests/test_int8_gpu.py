@@ -235,7 +235,8 @@ def test_products_however_cut(ops, m, n, k):
 # one row and two, in blocks of four warps and of eight, the last of them full and not
 @pytest.mark.parametrize("silu", [False, True], ids=["plain", "gated"])
 @pytest.mark.parametrize("n,k", [(2, 16), (34, 8208), (3500, 528), (3560, 528), (5120, 5120), (6002, 1040), (7102, 2064), (7110, 2064),
-                                 (8190, 2576), (10654, 2064), (10660, 2064), (24002, 272)])
+                                 (2662, 1040), (2668, 1040), (5326, 2064), (5334, 2064), (7990, 2064), (7998, 2064), (8190, 2576),
+                                 (10654, 2064), (10660, 2064), (24002, 272)])
 def test_single_rows(ops, n, k, silu):
     a, sa, w, sw, bias = (t.cuda() for t in _case(2, n, k, BF16, True))
     for m in (1, 2):

@@ -650,7 +650,7 @@ split_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
 // turn, `kRows` 16-byte loads a lane at once, four products per dp4a.  Blocks are small and many per SM, so that enough loads are under
 // way and the last ones end together: four warps, or eight (WIDE) as `wide_rows` says.
 template <int MT, bool WIDE> struct Gemv {
-  static constexpr int kThreads = WIDE ? 256 : 128, kRows = WIDE ? 6 : 8, kPerSm = WIDE ? 4 : MT == 1 ? 6 : 5;
+  static constexpr int kThreads = WIDE ? 256 : 128, kRows = WIDE ? 6 : MT == 1 ? 8 : 4, kPerSm = WIDE ? 5 - MT : MT == 1 ? 6 : 9;
 };
 
 template <int OUT, bool SILU, int MT, bool WIDE>
@@ -863,14 +863,22 @@ static void launch_gemv(const Args& g, cudaStream_t st) {
   B200_CUDA_LAUNCH_CHECK();
 }
 
-// One row: blocks of eight warps where those of four would be too few to fill half the chip, or would leave the second of two turns
-// mostly empty.  us, four warps and eight: 4 096 x 14 336 10.2 and 11.6, 6 144 x 4 096 4.9 and 5.6, 28 672 x 4 096 18.9 and 20.0,
+// Blocks of eight warps where those of four would be too few to fill half the chip, or would leave the second of two turns mostly
+// empty.  us, four warps and eight, one row: 4 096 x 14 336 10.2 and 11.6, 6 144 x 4 096 4.9 and 5.6, 28 672 x 4 096 18.9 and 20.0,
 // 5 120 x 5 120 5.5 and 6.8, 151 936 x 2 048 45.5 and 65.9, 8 192 x 2 048 4.4 and 4.9; but 1 024 x 8 192 4.6 and 3.4, 2 560 x 6 144 4.4
 // and 4.0, 8 192 x 4 096 7.6 and 6.7, 10 240 x 8 192 15.1 and 13.7, 8 192 x 28 672 39.3 and 35.9.  In later turns, 14 336 to 57 344
-// channels, the two are within 5 % at K from 7 168.
-static bool wide_rows(const Args& g) {
-  const int64_t blocks = (g.N - 1) / Gemv<1, false>::kRows + 1, at_once = static_cast<int64_t>(Gemv<1, false>::kPerSm) * sm_count();
+// channels, the two are within 5 % at K from 7 168.  Two rows: 4 096 x 14 336 9.9 and 11.0, 5 120 x 5 120 5.5 and 6.4, 28 672 x 4 096
+// gated 20.4 and 24.3 (8 rows to four warps 10.5, 5.6 and 20.2); but 1 024 x 8 192 4.3 and 3.3, 2 560 x 6 912 4.9 and 4.2, 6 144 x 4 096
+// 6.4 and 6.0.
+template <int MT> static bool wide_rows(const Args& g) {
+  const int64_t blocks = (g.N - 1) / Gemv<MT, false>::kRows + 1, at_once = static_cast<int64_t>(Gemv<MT, false>::kPerSm) * sm_count();
   return blocks * 2 < at_once || (g.K > 2048 && blocks > at_once && blocks * 2 < at_once * 3);
+}
+
+template <int OUT, bool SILU, int MT>
+static void launch_gemv(const Args& g, cudaStream_t st) {
+  if (wide_rows<MT>(g)) launch_gemv<OUT, SILU, MT, true>(g, st);
+  else launch_gemv<OUT, SILU, MT, false>(g, st);
 }
 
 // Shared memory that a block asks for at least, so that the blocks on an SM never want more tensor memory together than there is: a
@@ -1016,8 +1024,8 @@ static void launch(const Args& g, cudaStream_t st) {
   // What goes without shared and tensor memory, us, against the split kernel: one row of 6 144 x 4 096 5.7 and 8.5, 28 672 x 4 096 gated
   // 20.3 and 21.5; two rows 6.8 and 8.6, 20.3 and 21.4; eight rows of 4 096 x 4 096 4.5 and 7.0, 6 144 x 4 096 6.5 and 8.3, 28 672 x
   // 4 096 gated 21.8 and 21.6, 57 344 x 8 192 gated 73.0 and 82.8; sixteen rows 5.7 and 7.2, 6.7 and 8.3, but 4 096 x 14 336 13.7 and 13.6.
-  if (g.M == 1) return wide_rows(g) ? launch_gemv<OUT, SILU, 1, true>(g, st) : launch_gemv<OUT, SILU, 1, false>(g, st);
-  if (g.M == 2) return launch_gemv<OUT, SILU, 2, false>(g, st);
+  if (g.M == 1) return launch_gemv<OUT, SILU, 1>(g, st);
+  if (g.M == 2) return launch_gemv<OUT, SILU, 2>(g, st);
   if (g.M <= 8) return launch_few<OUT, SILU, 1>(g, st);
   if (g.M <= 16 && static_cast<int64_t>(g.N) * g.K <= 32 << 20) return launch_few<OUT, SILU, 2>(g, st);
   const Plan p = plan(g);
