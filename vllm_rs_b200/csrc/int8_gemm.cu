@@ -1021,9 +1021,10 @@ static void launch_few(const Args& g, cudaStream_t st) {
 
 template <int OUT, bool SILU>
 static void launch(const Args& g, cudaStream_t st) {
-  // What goes without shared and tensor memory, us, against the split kernel: one row of 6 144 x 4 096 5.7 and 8.5, 28 672 x 4 096 gated
-  // 20.3 and 21.5; two rows 6.8 and 8.6, 20.3 and 21.4; eight rows of 4 096 x 4 096 4.5 and 7.0, 6 144 x 4 096 6.5 and 8.3, 28 672 x
-  // 4 096 gated 21.8 and 21.6, 57 344 x 8 192 gated 73.0 and 82.8; sixteen rows 5.7 and 7.2, 6.7 and 8.3, but 4 096 x 14 336 13.7 and 13.6.
+  // What goes without shared and tensor memory, us, against the split kernel: one row of 6 144 x 4 096 4.9 and 8.5, 28 672 x 4 096 gated
+  // 19.3 and 22.1; two rows 5.9 and 8.5, 20.4 and 21.5; eight rows of 4 096 x 4 096 4.4 and 6.3, 6 144 x 4 096 6.5 and 8.2, 4 096 x
+  // 14 336 11.2 and 13.3, 8 192 x 8 192 13.7 and 14.1, 57 344 x 8 192 gated 74.8 and 74.3, 8 192 x 28 672 39.7 and 37.6; sixteen rows of
+  // 4 096 x 4 096 5.6 and 6.4, 6 144 x 4 096 6.6 and 8.3, but 4 096 x 14 336 13.7 and 13.3.
   if (g.M == 1) return launch_gemv<OUT, SILU, 1>(g, st);
   if (g.M == 2) return launch_gemv<OUT, SILU, 2>(g, st);
   if (g.M <= 8) return launch_few<OUT, SILU, 1>(g, st);
